@@ -371,6 +371,92 @@ int b2a_proj(const void* x, int64_t x_row_stride, int M, int K, const void* w, i
              float eps, const void* res, int64_t res_row_stride, void* out, int64_t out_row_stride, int mode,
              int dtype, void* stream);
 
+/* ------------------------------------------------------------------------
+ * 4-bit KV pool (no counterpart in the reference).
+ * A pool of num_slots token rows of b2a_fp4_row_bytes(Hkv, D) bytes each (0 for
+ * a shape that is not supported; D is 64, 128 or 256), 16-byte aligned, zeroed
+ * once when it is allocated. A head row is cut into blocks of 16 features with
+ *   s    = e4m3(min(max|x| / 6, 448))   one byte
+ *   code = e2m1(x / s)                  four bits: +-{0, .5, 1, 1.5, 2, 3, 4, 6}
+ * both to nearest, ties to even, clipped at their ends; x is the element divided
+ * by k_scale (v_scale), a power of two in [2^-100, 2^100], and the stored value
+ * stands for code * s * k_scale (v_scale). A row holds, for each kv head, the
+ * codes of K (D/2 bytes, feature 2i in the low nibble of byte i) and of V, then,
+ * for each kv head, the scales of K (D/16 bytes) and of V, then padding. A NaN
+ * is stored as 0 and does not count for the maximum, an infinity is clipped: the
+ * pool holds finite values only.
+ *
+ * b2a_fp4_store_kv quantises T rows of k and v (row strides in elements) into
+ * slots out_loc, which must be unique. dtype f32, bf16 or f16; rows of any
+ * alignment. b2a_fp4_load_kv expands the rows of n slots into contiguous
+ * [n, Hkv, D] k_out and v_out, exactly for f32 and bf16 (f16 holds every value
+ * while k_scale and v_scale are 1). A slot outside the pool is recorded as device
+ * error 32; the store skips it, the load returns zeros for it.
+ * ------------------------------------------------------------------------ */
+size_t b2a_fp4_row_bytes(int Hkv, int D);
+int b2a_fp4_store_kv(const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, const int32_t* out_loc,
+                     void* pool, int64_t num_slots, int64_t T, int Hkv, int D, float k_scale, float v_scale, int dtype,
+                     void* stream);
+int b2a_fp4_load_kv(const void* pool, int64_t num_slots, const int32_t* slots, int64_t n, int Hkv, int D,
+                    float k_scale, float v_scale, void* k_out, void* v_out, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged split-KV decode attention over the 4-bit pool: b2a_decode (its plan,
+ * workspace, launch order and device errors) on the values b2a_fp4_load_kv
+ * returns. q and out are f32 or bf16 [B, Hq, D]; Hkv in {1, 2, 4, 8, 16}, any
+ * GQA group up to 8, any power-of-two page size up to 4096. scale is positive
+ * and finite. A request without tokens gets a row of zeros. The plan comes from
+ * b2a_decode_plan or b2a_decode_metadata with b2a_fp4_decode_num_ctas CTAs.
+ * ------------------------------------------------------------------------ */
+int b2a_fp4_decode_num_ctas(int Hq, int Hkv, int D, int dtype, int* num_ctas);
+int b2a_fp4_decode(const void* q, const void* pool, int64_t num_slots, const int32_t* kv_indices, int page_size,
+                   const int32_t* cta_indptr, const int32_t* segs, int num_ctas, const int32_t* merge_indptr,
+                   int n_partials, int B, int Hq, int Hkv, int D, float scale, float k_scale, float v_scale,
+                   void* workspace, size_t workspace_bytes, void* out, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Ragged causal extend (prefill) attention over the 4-bit pool: b2a_extend on
+ * the values b2a_fp4_load_kv returns, for any power-of-two page size. q and out
+ * are f32 or bf16 [T, Hq, D], GQA group 1, 2, 4 or 8. `work` comes from
+ * b2a_extend_plan or b2a_extend_metadata with the tile size that
+ * b2a_fp4_extend_tile_q returns for the same shape; empty tiles at its end are
+ * skipped. scale is positive and finite.
+ * ------------------------------------------------------------------------ */
+int b2a_fp4_extend_tile_q(int Hq, int Hkv, int D, int dtype, int* tile_q);
+int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int32_t* qo_indptr,
+                   const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* kv_last_page_len, int page_size,
+                   const int32_t* work, int n_work, int T, int B, int Hq, int Hkv, int D, float scale, float k_scale,
+                   float v_scale, void* out, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Prefill tables built on the device (stream-ordered, no host work, capturable
+ * in a CUDA graph). Replaces the per-batch host build of _prepare_prefill
+ * (python/minisgl_mlx/attention/base.py:70-84), the positions / out_loc lookup
+ * of scheduler/scheduler.py:155-158 and b2a_extend_plan. Request b has lens[b]
+ * tokens, the first cached[b] of them in the pool already:
+ *   page_table    : device int32 [table_rows, table_stride], token-granular
+ *   rows, cached, lens : device int32 [B]
+ *   qo_indptr     : out int32 [B + 1]        CSR over new tokens
+ *   positions, out_loc : out int32 [q_capacity] position and pool slot of every new token
+ *   last_indices  : out int32 [B]            qo_indptr[b + 1] - 1
+ *   kv_indptr, kv_indices [idx_capacity], kv_last_page_len : out, page CSR
+ *   work          : out int32 [work_capacity * 4], b2a_extend_plan's list for
+ *                   tile_q (at most 256), then empty tiles {0, 0, 0, 0}; 16-byte
+ *                   aligned; min(B, T) + T / tile_q entries are always enough
+ *   counts        : out int32 [2] = {new tokens, tiles}
+ * Identical values to the host builders. Entries past what the batch needs are
+ * left as they were (except work). B <= 8192. Lengths outside [0, table_stride],
+ * cached lengths outside [0, lens[b]], rows outside the table and entries past a
+ * capacity are skipped and recorded as device error 34 (b2a_device_error),
+ * negative or unaligned page entries as 32; a work list that does not fit is
+ * left empty.
+ * ------------------------------------------------------------------------ */
+int b2a_extend_metadata(const int32_t* page_table, int64_t table_rows, int64_t table_stride, const int32_t* rows,
+                        const int32_t* cached, const int32_t* lens, int B, int page_size, int tile_q,
+                        int32_t* qo_indptr, int32_t* positions, int32_t* out_loc, int64_t q_capacity,
+                        int32_t* last_indices, int32_t* kv_indptr, int32_t* kv_indices, int64_t idx_capacity,
+                        int32_t* kv_last_page_len, int32_t* work, int work_capacity, int32_t* counts, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,9 +16,12 @@
 #include "b200attn.h"
 #include "common.cuh"
 #include "decode.cuh"
+#include "decode_fp4.cuh"
 #include "decode_mma.cuh"
+#include "extend_meta.cuh"
 #include "extend_simt.cuh"
 #include "extend_tc.cuh"
+#include "fp4_kv.cuh"
 #include "pack_kv.cuh"
 #include "proj.cuh"
 #include "metadata.cuh"
@@ -1066,3 +1069,336 @@ extern "C" int b2a_proj(const void* x, int64_t x_row_stride, int M, int K, const
   if (M <= 32) return proj_tiles<4>(a, mode, norm, grid, st);
   return proj_tiles<8>(a, mode, norm, grid, st);
 }
+
+// ------------------------------------------------------------------ 4-bit KV pool
+namespace {
+
+bool power_of_two(float x) {
+  uint32_t b;
+  std::memcpy(&b, &x, 4);
+  return x > 0.f && (b & 0x7fffffu) == 0 && (b >> 23) >= 27 && (b >> 23) <= 227;  // 2^-100 .. 2^100
+}
+
+int fp4_check(int Hkv, int D, float k_scale, float v_scale) {
+  if (Hkv <= 0 || D <= 0) return fail(B2A_ERR_INVALID, "head counts and head_dim must be > 0");
+  if (D != 64 && D != 128 && D != 256) return fail(B2A_ERR_UNSUPPORTED, "fp4: head_dim %d (64, 128, 256)", D);
+  if (Hkv > 1024) return fail(B2A_ERR_UNSUPPORTED, "fp4: Hkv = %d (at most 1024)", Hkv);
+  if (!power_of_two(k_scale) || !power_of_two(v_scale))
+    return fail(B2A_ERR_INVALID, "fp4: k_scale and v_scale must be powers of two in [2^-100, 2^100]");
+  return B2A_OK;
+}
+
+// The decode kernel's launch shape for the 4-bit pool.
+int fp4_decode_config(int Hq, int Hkv, int D, DecodeCfg& c) {
+  const int G = Hq / Hkv;
+  if (Hkv > 16 || 16 % Hkv != 0)
+    return fail(B2A_ERR_UNSUPPORTED, "fp4 decode supports Hkv in {1, 2, 4, 8, 16}, got %d", Hkv);
+  if (G > 8) return fail(B2A_ERR_UNSUPPORTED, "fp4 decode: GQA group %d (at most 8)", G);
+  c.row_bytes = b2a::fp4_row_bytes(Hkv, D);
+  // 16 consumer warps; 8 at head_dim 256, whose accumulators need more than the ~118
+  // registers 17 warps leave a thread (16 kv heads still take a warp each)
+  c.NCW = (D == 256 && Hkv < 16) ? 8 : 16;
+  c.WPH = c.NCW / Hkv;
+  // a stage holds a unit of 16 tokens for every warp, more while it stays near 40 KB
+  c.TS = b2a::kFp4Tok * c.WPH;
+  while (2u * c.TS * c.row_bytes <= 40960u) c.TS *= 2;
+  c.stage_bytes = (uint32_t)c.TS * c.row_bytes;
+  const size_t fixed = b2a::fp4_decode_smem(0, c.stage_bytes, c.NCW, c.WPH, G, D).total + 6 * 16;
+  c.NSTAGE = (int)std::min<size_t>(6, (kSmemLimit - fixed) / c.stage_bytes);
+  if (c.NSTAGE < 2) return fail(B2A_ERR_UNSUPPORTED, "fp4 decode (Hq %d, Hkv %d, D %d) does not fit", Hq, Hkv, D);
+  c.smem = b2a::fp4_decode_smem(c.NSTAGE, c.stage_bytes, c.NCW, c.WPH, G, D).total;
+  return B2A_OK;
+}
+
+template <typename T, int D, int NCW>
+int fp4_decode_launch(const b2a::DecodeArgs& a, const DecodeCfg& c, float v_scale, int grid, cudaStream_t st) {
+  auto kern = b2a::decode_fp4_kernel<T, D, NCW>;
+  if (int rc = ensure_smem((const void*)kern, c.smem, "fp4_decode")) return rc;
+  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3((NCW + 1) * 32), c.smem, st, a, v_scale);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(B2A_ERR_CUDA, "decode_fp4_kernel: %s", cudaGetErrorString(e));
+  }
+  return check_launch("decode_fp4_kernel");
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t b2a_fp4_row_bytes(int Hkv, int D) {
+  if (Hkv <= 0 || Hkv > 1024 || (D != 64 && D != 128 && D != 256)) return 0;
+  return b2a::fp4_row_bytes(Hkv, D);
+}
+
+int b2a_fp4_store_kv(const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, const int32_t* out_loc,
+                     void* pool, int64_t num_slots, int64_t T, int Hkv, int D, float k_scale, float v_scale, int dtype,
+                     void* stream) {
+  if (T < 0) return fail(B2A_ERR_INVALID, "T must be >= 0");
+  if (int rc = fp4_check(Hkv, D, k_scale, v_scale)) return rc;
+  const size_t es = dtype_size(dtype);
+  if (es == 0) return fail(B2A_ERR_INVALID, "unknown dtype code %d", dtype);
+  if (T == 0) return ok();
+  if (!k || !v || !out_loc || !pool) return fail(B2A_ERR_INVALID, "NULL pointer argument");
+  if (num_slots <= 0) return fail(B2A_ERR_INVALID, "num_slots must be > 0");
+  if (k_row_stride < (int64_t)Hkv * D || v_row_stride < (int64_t)Hkv * D)
+    return fail(B2A_ERR_INVALID, "row strides smaller than a token row");
+  if (!aligned(pool, 16) || !aligned(k, es) || !aligned(v, es))
+    return fail(B2A_ERR_INVALID, "pool must be 16-byte aligned, k and v to their element size");
+  b2a::Fp4KvArgs a = {};
+  a.k = k;
+  a.v = v;
+  a.k_stride = k_row_stride;
+  a.v_stride = v_row_stride;
+  a.slots = out_loc;
+  a.pool = reinterpret_cast<uint8_t*>(pool);
+  a.num_slots = num_slots;
+  a.n = T;
+  a.Hkv = Hkv;
+  a.nblk = D / b2a::kFp4Block;
+  a.row_bytes = b2a::fp4_row_bytes(Hkv, D);
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  const int64_t blocks = (T * 2 * Hkv * a.nblk + 255) / 256;
+  if (blocks > 0x7fffffff) return fail(B2A_ERR_INVALID, "too many rows");
+  const bool vec = aligned(k, 16) && aligned(v, 16) && (k_row_stride * (int64_t)es) % 16 == 0 &&
+                   (v_row_stride * (int64_t)es) % 16 == 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return with_dtype<true>(dtype, [&](auto tag) -> int {
+    using Tt = decltype(tag);
+    if (vec) launch_pdl(b2a::fp4_store_kernel<Tt, true>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    else launch_pdl(b2a::fp4_store_kernel<Tt, false>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    return check_launch("fp4_store_kernel");
+  });
+}
+
+int b2a_fp4_load_kv(const void* pool, int64_t num_slots, const int32_t* slots, int64_t n, int Hkv, int D,
+                    float k_scale, float v_scale, void* k_out, void* v_out, int dtype, void* stream) {
+  if (n < 0) return fail(B2A_ERR_INVALID, "n must be >= 0");
+  if (int rc = fp4_check(Hkv, D, k_scale, v_scale)) return rc;
+  if (dtype_size(dtype) == 0) return fail(B2A_ERR_INVALID, "unknown dtype code %d", dtype);
+  if (n == 0) return ok();
+  if (!pool || !slots || !k_out || !v_out) return fail(B2A_ERR_INVALID, "NULL pointer argument");
+  if (num_slots <= 0) return fail(B2A_ERR_INVALID, "num_slots must be > 0");
+  if (!aligned(pool, 16) || !aligned(k_out, 16) || !aligned(v_out, 16))
+    return fail(B2A_ERR_INVALID, "pool, k_out and v_out must be 16-byte aligned");
+  b2a::Fp4KvArgs a = {};
+  a.k_out = k_out;
+  a.v_out = v_out;
+  a.slots = slots;
+  a.pool = const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(pool));
+  a.num_slots = num_slots;
+  a.n = n;
+  a.Hkv = Hkv;
+  a.nblk = D / b2a::kFp4Block;
+  a.row_bytes = b2a::fp4_row_bytes(Hkv, D);
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  const int64_t blocks = (n * 2 * Hkv * a.nblk + 255) / 256;
+  if (blocks > 0x7fffffff) return fail(B2A_ERR_INVALID, "too many rows");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return with_dtype<true>(dtype, [&](auto tag) -> int {
+    using Tt = decltype(tag);
+    launch_pdl(b2a::fp4_load_kernel<Tt>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    return check_launch("fp4_load_kernel");
+  });
+}
+
+int b2a_fp4_decode_num_ctas(int Hq, int Hkv, int D, int dtype, int* num_ctas) {
+  if (!num_ctas) return fail(B2A_ERR_INVALID, "num_ctas is NULL");
+  if (int rc = check_heads(Hq, Hkv, D)) return rc;
+  if (int rc = fp4_check(Hkv, D, 1.f, 1.f)) return rc;
+  if (dtype != B2A_DTYPE_F32 && dtype != B2A_DTYPE_BF16) return fail(B2A_ERR_UNSUPPORTED, "fp4 decode dtype %d", dtype);
+  DecodeCfg c;
+  if (int rc = fp4_decode_config(Hq, Hkv, D, c)) return rc;
+  const int sms = num_sms();
+  if (sms <= 0) return fail(B2A_ERR_CUDA, "no CUDA device");
+  *num_ctas = sms;  // the stages of one CTA take an SM's shared memory
+  return ok();
+}
+
+int b2a_fp4_decode(const void* q, const void* pool, int64_t num_slots, const int32_t* kv_indices, int page_size,
+                   const int32_t* cta_indptr, const int32_t* segs, int num_ctas, const int32_t* merge_indptr,
+                   int n_partials, int B, int Hq, int Hkv, int D, float scale, float k_scale, float v_scale,
+                   void* workspace, size_t workspace_bytes, void* out, int dtype, void* stream) {
+  if (B < 0) return fail(B2A_ERR_INVALID, "B must be >= 0");
+  if (int rc = check_heads(Hq, Hkv, D)) return rc;
+  if (int rc = fp4_check(Hkv, D, k_scale, v_scale)) return rc;
+  if (dtype != B2A_DTYPE_F32 && dtype != B2A_DTYPE_BF16) return fail(B2A_ERR_UNSUPPORTED, "fp4 decode dtype %d", dtype);
+  if (!(scale > 0.f) || scale > 1e30f) return fail(B2A_ERR_INVALID, "fp4 decode: scale must be positive and finite");
+  if (B == 0) return ok();
+  if (!cta_indptr || !segs || num_ctas <= 0) return fail(B2A_ERR_INVALID, "decode plan missing (cta_indptr/segs)");
+  if (!aligned(segs, 16)) return fail(B2A_ERR_INVALID, "segs must be 16-byte aligned (read as int4)");
+  if (!q || !pool || !kv_indices || !out) return fail(B2A_ERR_INVALID, "NULL tensor pointer");
+  if (num_slots <= 0) return fail(B2A_ERR_INVALID, "num_slots must be > 0");
+  if (!aligned(q, 16) || !aligned(pool, 16) || !aligned(out, 16))
+    return fail(B2A_ERR_INVALID, "q/pool/out must be 16-byte aligned");
+  const int plog = ilog2_exact(page_size);
+  if (plog < 0 || page_size > 4096) return fail(B2A_ERR_INVALID, "page_size %d must be a power of two <= 4096", page_size);
+  DecodeCfg c;
+  if (int rc = fp4_decode_config(Hq, Hkv, D, c)) return rc;
+  if (n_partials < 0) return fail(B2A_ERR_INVALID, "n_partials must be >= 0");
+  const size_t need = b2a_decode_workspace_bytes(n_partials, Hq, D);
+  if (n_partials > 0 && (!workspace || workspace_bytes < need || !merge_indptr))
+    return fail(B2A_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  if (workspace && !aligned(workspace, 256)) return fail(B2A_ERR_INVALID, "workspace must be 256-byte aligned");
+  b2a::DecodeArgs a = {};
+  a.q = q;
+  a.k_pool = pool;
+  a.kv_indices = kv_indices;
+  a.num_slots = num_slots;
+  a.cta_indptr = cta_indptr;
+  a.segs = segs;
+  a.merge_indptr = merge_indptr;
+  if (n_partials > 0) {
+    const DecodeWs w = decode_ws_layout(workspace, workspace_bytes, n_partials, Hq, D);
+    a.tickets = w.tickets;
+    a.ws_acc = w.acc;
+    a.ws_ml = w.ml;
+  }
+  a.B = B;
+  a.n_partials = n_partials;
+  a.out = out;
+  a.page_log2 = plog;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.qscale = scale * k_scale * b2a::kLog2e;
+  a.TS = c.TS;
+  a.NSTAGE = c.NSTAGE;
+  a.WPH = c.WPH;
+  a.NCW = c.NCW;
+  a.row_bytes = c.row_bytes;
+  a.stage_bytes = c.stage_bytes;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return with_dtype<false>(dtype, [&](auto tag) -> int {
+    using Tt = decltype(tag);
+    switch (D) {
+      case 64:
+        return fp4_decode_launch<Tt, 64, 16>(a, c, v_scale, num_ctas, st);
+      case 128:
+        return fp4_decode_launch<Tt, 128, 16>(a, c, v_scale, num_ctas, st);
+      default:
+        return c.NCW == 16 ? fp4_decode_launch<Tt, 256, 16>(a, c, v_scale, num_ctas, st)
+                           : fp4_decode_launch<Tt, 256, 8>(a, c, v_scale, num_ctas, st);
+    }
+  });
+}
+
+int b2a_fp4_extend_tile_q(int Hq, int Hkv, int D, int dtype, int* tile_q) {
+  if (!tile_q) return fail(B2A_ERR_INVALID, "tile_q is NULL");
+  if (int rc = check_heads(Hq, Hkv, D)) return rc;
+  if (int rc = fp4_check(Hkv, D, 1.f, 1.f)) return rc;
+  if (dtype != B2A_DTYPE_F32 && dtype != B2A_DTYPE_BF16) return fail(B2A_ERR_UNSUPPORTED, "fp4 extend dtype %d", dtype);
+  const int G = Hq / Hkv;
+  if (G != 1 && G != 2 && G != 4 && G != 8) return fail(B2A_ERR_UNSUPPORTED, "GQA group size %d not compiled (1, 2, 4, 8)", G);
+  *tile_q = b2a::kSimtRows / G;
+  return ok();
+}
+
+int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int32_t* qo_indptr,
+                   const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* kv_last_page_len, int page_size,
+                   const int32_t* work, int n_work, int T, int B, int Hq, int Hkv, int D, float scale, float k_scale,
+                   float v_scale, void* out, int dtype, void* stream) {
+  if (n_work < 0 || B < 0 || T < 0) return fail(B2A_ERR_INVALID, "negative size");
+  if (int rc = check_heads(Hq, Hkv, D)) return rc;
+  if (int rc = fp4_check(Hkv, D, k_scale, v_scale)) return rc;
+  if (dtype != B2A_DTYPE_F32 && dtype != B2A_DTYPE_BF16) return fail(B2A_ERR_UNSUPPORTED, "fp4 extend dtype %d", dtype);
+  if (!(scale > 0.f) || scale > 1e30f) return fail(B2A_ERR_INVALID, "fp4 extend: scale must be positive and finite");
+  const int plog = ilog2_exact(page_size);
+  if (plog < 0) return fail(B2A_ERR_INVALID, "page_size %d must be a power of two", page_size);
+  if (n_work == 0 || B == 0 || T == 0) return ok();
+  if (!q || !pool || !qo_indptr || !kv_indptr || !kv_indices || !work || !out)
+    return fail(B2A_ERR_INVALID, "NULL pointer argument");
+  if (!aligned(work, 16)) return fail(B2A_ERR_INVALID, "work must be 16-byte aligned (read as int4)");
+  if (!aligned(q, 16) || !aligned(pool, 16) || !aligned(out, 16))
+    return fail(B2A_ERR_INVALID, "q/pool/out must be 16-byte aligned");
+  if (num_slots <= 0) return fail(B2A_ERR_INVALID, "num_slots must be > 0");
+  if (Hkv > 65535) return fail(B2A_ERR_UNSUPPORTED, "too many kv heads");
+  const int G = Hq / Hkv;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  b2a::ExtendArgs a = {};
+  a.q = q;
+  a.k_pool = pool;
+  a.qo_indptr = qo_indptr;
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.kv_last_page_len = kv_last_page_len;
+  a.work = work;
+  a.out = out;
+  a.num_slots = num_slots;
+  a.page_log2 = plog;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.qscale = scale * k_scale * b2a::kLog2e;
+  a.row_bytes = (int)b2a::fp4_row_bytes(Hkv, D);
+  a.v_scale = v_scale;
+  return with_dtype<false>(dtype, [&](auto tag) -> int {
+    using Tt = decltype(tag);
+    return with_d(D, [&](auto dc) -> int {
+      constexpr int Dc = decltype(dc)::value;
+      return with_g<Dc>(G, [&](auto gc) -> int {
+        constexpr int Gc = decltype(gc)::value;
+        auto kern = b2a::extend_simt_kernel<Tt, Dc, Gc, true>;
+        const size_t smem = b2a::extend_simt_smem(Dc);
+        if (int rc = ensure_smem((const void*)kern, smem, "fp4_extend")) return rc;
+        kern<<<dim3(n_work, Hkv), b2a::kSimtThreads, smem, st>>>(a);
+        return check_launch("extend_simt_kernel (fp4)");
+      });
+    });
+  });
+}
+
+// ------------------------------------------------------------------ prefill tables
+int b2a_extend_metadata(const int32_t* page_table, int64_t table_rows, int64_t table_stride, const int32_t* rows,
+                        const int32_t* cached, const int32_t* lens, int B, int page_size, int tile_q,
+                        int32_t* qo_indptr, int32_t* positions, int32_t* out_loc, int64_t q_capacity,
+                        int32_t* last_indices, int32_t* kv_indptr, int32_t* kv_indices, int64_t idx_capacity,
+                        int32_t* kv_last_page_len, int32_t* work, int work_capacity, int32_t* counts, void* stream) {
+  if (B < 0) return fail(B2A_ERR_INVALID, "B must be >= 0");
+  if (B > b2a::kEmMaxBatch) return fail(B2A_ERR_UNSUPPORTED, "B = %d requests (at most %d)", B, b2a::kEmMaxBatch);
+  const int plog = ilog2_exact(page_size);
+  if (plog < 0) return fail(B2A_ERR_INVALID, "page_size %d must be a power of two", page_size);
+  if (tile_q <= 0 || tile_q > b2a::kEmMaxTile)
+    return fail(B2A_ERR_INVALID, "tile_q %d out of [1, %d]", tile_q, b2a::kEmMaxTile);
+  if (table_rows <= 0 || table_stride <= 0 || table_stride > 0x7fffffffLL)
+    return fail(B2A_ERR_INVALID, "page table of %lld x %lld", (long long)table_rows, (long long)table_stride);
+  if (q_capacity < 0 || idx_capacity < 0 || work_capacity < 0 || work_capacity > b2a::kEmMaxWork)
+    return fail(B2A_ERR_INVALID, "capacities must be >= 0 (work at most %d)", b2a::kEmMaxWork);
+  if (!page_table || !qo_indptr || !kv_indptr || !counts ||
+      (B > 0 && (!rows || !cached || !lens || !last_indices || !kv_last_page_len)) ||
+      (q_capacity > 0 && (!positions || !out_loc)) || (idx_capacity > 0 && !kv_indices) || (work_capacity > 0 && !work))
+    return fail(B2A_ERR_INVALID, "NULL metadata argument");
+  if (!aligned(work, 16)) return fail(B2A_ERR_INVALID, "work must be 16-byte aligned (written as int4)");
+  b2a::ExtendMetaArgs a;
+  a.page_table = page_table;
+  a.stride = table_stride;
+  a.table_rows = table_rows;
+  a.rows = rows;
+  a.cached = cached;
+  a.lens = lens;
+  a.B = B;
+  a.page_log2 = plog;
+  a.tile_q = tile_q;
+  a.qo_indptr = qo_indptr;
+  a.positions = positions;
+  a.out_loc = out_loc;
+  a.q_capacity = q_capacity;
+  a.last_indices = last_indices;
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.idx_capacity = idx_capacity;
+  a.last_page_len = kv_last_page_len;
+  a.work = work;
+  a.work_capacity = work_capacity;
+  a.counts = counts;
+  const size_t smem = b2a::extend_meta_smem(B);
+  if (int rc = ensure_smem((const void*)b2a::extend_meta_kernel, b2a::extend_meta_smem(b2a::kEmMaxBatch), "extend_meta"))
+    return rc;
+  // enough threads for one walk each over tokens and pages, at most two CTAs per SM
+  const int64_t walks = (std::max(q_capacity, idx_capacity) + b2a::kEmVec - 1) / b2a::kEmVec;
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(2 * 148, (walks + b2a::kEmThreads - 1) / b2a::kEmThreads));
+  b2a::extend_meta_kernel<<<(unsigned)grid, b2a::kEmThreads, smem, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+  return check_launch("extend_meta_kernel");
+}
+
+}  // extern "C"

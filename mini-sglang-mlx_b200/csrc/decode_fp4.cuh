@@ -1,0 +1,522 @@
+// Paged decode attention over the 4-bit KV pool (one query row per request).
+//
+//   out[b, h] = softmax(scale * q[b, h] . K^T) . V,   K, V = code * s of fp4_kv.cuh
+//
+// Same plan, workspace, in-launch merge and error handling as decode_kernel
+// (decode.cuh): a persistent grid, each CTA an equal share of the batch's page
+// stream, one producer warp that brings whole token rows with bulk copies.
+//
+// What bounds it. A cached value is 0.56 bytes, so at HBM rate an SM receives
+// about 40 values per clock (1.13 bytes and 2 G multiply-adds per K/V pair):
+// expanding and multiplying them has to cost less than a clock per 40 values.
+// One warp takes units of 16 tokens x one kv head:
+//   S^T [16 tokens x 8 head columns] = K [16 x D] . Q^T      (D/16 MMAs)
+//   O^T [D x 8]                     += V^T [D x 16] . P^T    (D/16 MMAs)
+// with mma.sync m16n8k16, fp16 in, fp32 accumulate. The codes become MMA
+// operands in registers: two codes per conversion, one packed multiply by the
+// block's scale, exact in fp16. The k order of a product is free, so a lane
+// takes D/4 consecutive features of a K row (one 16-byte shared load at D =
+// 128), and Q is laid out to match; for V a lane takes D/8 consecutive features
+// of four tokens, and the codes of two tokens are interleaved in the word
+// before they are expanded, so an operand register holds one feature of two
+// tokens without any shuffle.
+//
+// q enters as fp16 with each head row scaled by a power of two so that its
+// largest element lies in [2^14, 2^15): bf16 has 8 significant bits, so only
+// elements 2^28 times smaller than the largest lose any. The factor goes back
+// through the softmax scale. fp32 q and P are split into two fp16 parts (22
+// bits). The lazy maximum of decode_mma.cuh (it moves when a score exceeds it by
+// more than 8) is kept 7 below the score that set it: weights lie in [0, 2^15] with
+// the largest at least 2^7, so a weight that fp16 holds as a subnormal is off by
+// at most 2^-32 of the largest. Softmax statistics and accumulators are fp32.
+#pragma once
+
+#include "decode.cuh"
+#include "decode_mma.cuh"
+#include "fp4_kv.cuh"
+
+namespace b2a {
+
+constexpr int kFp4Tok = 16;  // tokens of a unit
+
+struct Fp4DecodeSmem {
+  uint32_t bars, cbuf, abort_flag, last_flag, total;
+};
+
+__host__ __device__ inline Fp4DecodeSmem fp4_decode_smem(int NSTAGE, uint32_t stage_bytes, int NCW, int WPH, int G,
+                                                         int D) {
+  Fp4DecodeSmem L;
+  uint32_t off = (uint32_t)NSTAGE * stage_bytes;
+  off = (off + 15u) & ~15u;
+  L.bars = off;
+  off += (uint32_t)NSTAGE * 16u;
+  L.cbuf = off;
+  if (WPH > 1) off += (uint32_t)NCW * (uint32_t)G * (uint32_t)(D + 2) * 4u;
+  off = (off + 15u) & ~15u;
+  L.abort_flag = off;
+  L.last_flag = off + 16;
+  L.total = off + 32;
+  return L;
+}
+
+// D += A (16x16 fp16, row) . B (16x8 fp16, col), fp32 accumulate.
+__device__ __forceinline__ void mma_16816_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  __half2 p = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&p);
+}
+
+__device__ __forceinline__ float2 h2_to_f2(uint32_t x) { return __half22float2(*reinterpret_cast<__half2*>(&x)); }
+
+// Power of two that brings a row's largest magnitude into [2^14, 2^15), and its inverse.
+// Zero, infinite and NaN rows keep a factor of one.
+__device__ __forceinline__ void fp4_row_factor(float amax, float& f, float& inv) {
+  int e = (int)((__float_as_uint(amax) >> 23) & 0xff) - 127;
+  if (!(amax > 0.f) || e > 127) e = 14;
+  e = e < -100 ? -100 : e;
+  f = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+  inv = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+}
+
+// Words of codes a lane reads from one K row (D/4 features) and one V row (D/8 features).
+template <int N>
+__device__ __forceinline__ void fp4_lds(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x;
+      w[4 * i + 1] = v.y;
+      w[4 * i + 2] = v.z;
+      w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// One unit. row0: shared address of token 0's row; nt of its 16 tokens are real.
+// qf[p]: part p of Q^T (features of this lane's quarter, head column g).
+template <int D, int SPLIT>
+__device__ __forceinline__ void fp4_unit(const uint8_t* row0, uint32_t pitch, uint32_t code_off, uint32_t scale_off,
+                                         int nt, int lane, const float (&qs)[2], const uint32_t (&qf)[SPLIT][D / 16][2],
+                                         float (&acc)[D / 16][4], float (&mref)[2], float (&lsum)[2]) {
+  constexpr unsigned FULL = 0xffffffffu;
+  constexpr int KS = D / 16;  // MMAs of a product
+  const int g = lane >> 2, t = lane & 3;
+  // ---- S^T: rows g and g + 8, features [t D/4, (t+1) D/4)
+  float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+  {
+    const uint8_t* ra = row0 + (uint32_t)g * pitch;
+    const uint8_t* rb = ra + 8u * pitch;
+    uint32_t wa[D / 32], wb[D / 32];
+    fp4_lds<D / 32>(ra + code_off + t * (D / 8), wa);
+    fp4_lds<D / 32>(rb + code_off + t * (D / 8), wb);
+#pragma unroll
+    for (int q = 0; q < D / 64; ++q) {  // one block of 16 features: 2 words, 4 MMAs
+      const uint32_t sa8 = ra[scale_off + t * (D / 64) + q], sb8 = rb[scale_off + t * (D / 64) + q];
+      const uint32_t sa = fp4_scale2_to_h2(sa8 | (sa8 << 8)), sb = fp4_scale2_to_h2(sb8 | (sb8 << 8));
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        uint32_t xa[4], xb[4];
+        fp4_word_to_h2(wa[2 * q + w], xa);
+        fp4_word_to_h2(wb[2 * q + w], xb);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          xa[j] = h2_mul(xa[j], sa);
+          xb[j] = h2_mul(xb[j], sb);
+        }
+        const int k = 4 * q + 2 * w;
+#pragma unroll
+        for (int p = 0; p < SPLIT; ++p) {
+          mma_16816_f16(s0, xa[0], xb[0], xa[1], xb[1], qf[p][k][0], qf[p][k][1]);
+          mma_16816_f16(s1, xa[2], xb[2], xa[3], xb[3], qf[p][k + 1][0], qf[p][k + 1][1]);
+        }
+      }
+    }
+  }
+  // x[0]: (token g, column 2t) x[1]: (g, 2t+1) x[2]: (g+8, 2t) x[3]: (g+8, 2t+1)
+  float x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = (s0[i] + s1[i]) * qs[i & 1];
+  if (nt < kFp4Tok) {
+    if (g >= nt) x[0] = x[1] = kNegInf;
+    if (g + 8 >= nt) x[2] = x[3] = kNegInf;
+  }
+  const float cm[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+  const bool grow = cm[0] > mref[0] + 15.f || cm[1] > mref[1] + 15.f;
+  if (__any_sync(FULL, grow)) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      float v = cm[n];
+      v = fmaxf(v, __shfl_xor_sync(FULL, v, 4));
+      v = fmaxf(v, __shfl_xor_sync(FULL, v, 8));
+      v = fmaxf(v, __shfl_xor_sync(FULL, v, 16));
+      if (v > mref[n] + 15.f) {  // the same decision on every lane of the column
+        const float alpha = (mref[n] == kNegInf) ? 0.f : exp2f(mref[n] - (v - 7.f));
+        mref[n] = v - 7.f;
+        lsum[n] *= alpha;
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt) {
+          acc[mt][n] *= alpha;
+          acc[mt][2 + n] *= alpha;
+        }
+      }
+    }
+  }
+  float p[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = (x[i] == kNegInf) ? 0.f : exp2f(x[i] - mref[i & 1]);
+  lsum[0] += p[0] + p[2];
+  lsum[1] += p[1] + p[3];
+  uint32_t pb[SPLIT][2];
+  {
+    const uint32_t h0 = pack_h2(p[0], p[1]), h1 = pack_h2(p[2], p[3]);
+    pb[0][0] = movmatrix_trans(h0);  // tokens 0-7
+    pb[0][1] = movmatrix_trans(h1);  // tokens 8-15
+    if constexpr (SPLIT == 2) {
+      const float2 f0 = h2_to_f2(h0), f1 = h2_to_f2(h1);
+      pb[1][0] = movmatrix_trans(pack_h2(p[0] - f0.x, p[1] - f0.y));
+      pb[1][1] = movmatrix_trans(pack_h2(p[2] - f1.x, p[3] - f1.y));
+    }
+  }
+  // ---- O^T: features [g D/8, (g+1) D/8) of tokens 2t, 2t+1, 2t+8, 2t+9
+  {
+    constexpr int NW = D / 64;  // words of codes per token
+    uint32_t lo[2][NW], hi[2][NW], sc[2][D > 128 ? 2 : 1];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int ta = 2 * t + 8 * u;
+      const uint8_t* ra = row0 + (uint32_t)ta * pitch;
+      const uint8_t* rb = ra + pitch;
+      uint32_t wa[NW], wb[NW];
+      fp4_lds<NW>(ra + code_off + D / 2 + g * (D / 16), wa);
+      fp4_lds<NW>(rb + code_off + D / 2 + g * (D / 16), wb);
+#pragma unroll
+      for (int q = 0; q < (D > 128 ? 2 : 1); ++q) {
+        const uint32_t so = scale_off + D / 16 + (g * (D / 8)) / 16 + q;
+        // rows past the last token hold whatever the stage held before: a zero scale
+        // keeps their products finite (their weights are zero)
+        const uint32_t sa8 = ta < nt ? ra[so] : 0u, sb8 = ta + 1 < nt ? rb[so] : 0u;
+        sc[u][q] = fp4_scale2_to_h2(sa8 | (sb8 << 8));
+      }
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        // bytes of (token a, token b) codes: even features, odd features
+        lo[u][w] = (wa[w] & 0x0f0f0f0fu) | ((wb[w] & 0x0f0f0f0fu) << 4);
+        hi[u][w] = ((wa[w] >> 4) & 0x0f0f0f0fu) | (wb[w] & 0xf0f0f0f0u);
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      uint32_t l0[4], h0[4], l1[4], h1[4];
+      fp4_word_to_h2(lo[0][w], l0);
+      fp4_word_to_h2(hi[0][w], h0);
+      fp4_word_to_h2(lo[1][w], l1);
+      fp4_word_to_h2(hi[1][w], h1);
+      const int q = w >> 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t a0 = h2_mul(l0[j], sc[0][q]), a1 = h2_mul(h0[j], sc[0][q]);
+        const uint32_t a2 = h2_mul(l1[j], sc[1][q]), a3 = h2_mul(h1[j], sc[1][q]);
+#pragma unroll
+        for (int pp = 0; pp < SPLIT; ++pp) mma_16816_f16(acc[4 * w + j], a0, a1, a2, a3, pb[pp][0], pb[pp][1]);
+      }
+    }
+  }
+}
+
+template <typename T, int D, int NCW>
+__global__ void __launch_bounds__((NCW + 1) * 32, 1) decode_fp4_kernel(const DecodeArgs a, const float v_scale) {
+  // programmatic dependent launch exactly as decode_kernel: the plan and the page ids are
+  // read before the wait, everything the previous kernel may have written after it
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr int SPLIT = sizeof(T) == 4 ? 2 : 1;
+  constexpr int KS = D / 16;
+  constexpr unsigned FULL = 0xffffffffu;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int G = a.Hq / a.Hkv;
+  const Fp4DecodeSmem L = fp4_decode_smem(a.NSTAGE, a.stage_bytes, NCW, a.WPH, G, D);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bars);
+  uint64_t* empty = full + a.NSTAGE;
+  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L.abort_flag);
+  volatile int* s_last = reinterpret_cast<volatile int*>(smem + L.last_flag);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.NSTAGE; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], NCW);
+    }
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+
+  const int seg0 = a.cta_indptr[blockIdx.x];
+  const int seg1 = a.cta_indptr[blockIdx.x + 1];
+  const bool last_first = decode_last_first(a, seg0, seg1);
+  const int P = 1 << a.page_log2;
+  const int TS = a.TS;
+
+  if (warp == NCW) {
+    // ------------------------------------------------------------ producer
+    const uint64_t pol = l2_evict_first_policy();
+    const uint8_t* pool = reinterpret_cast<const uint8_t*>(a.k_pool);
+    const size_t rowB = a.row_bytes;
+    int ctr = 0;
+    bool ok = true;
+    bool waited = false;
+    for (int i = 0; i < seg1 - seg0 && ok; ++i) {
+      const int si = decode_seg_at(a, seg0, seg1, last_first, i);
+      int b, pbeg, ntok, slot;
+      decode_get_seg(a, si, b, pbeg, ntok, slot);
+      if (!decode_seg_ok(a, b, slot)) continue;  // the consumers skip it too (and report it)
+      for (int tok = 0; tok < ntok; tok += TS) {
+        if (!__all_sync(FULL, *s_abort == 0)) {
+          ok = false;
+          break;
+        }
+        const int nt = min(TS, ntok - tok);
+        const int st = ctr % a.NSTAGE;
+        const uint32_t ph = (uint32_t)(ctr / a.NSTAGE) & 1u;
+        if (!__all_sync(FULL, mbar_wait(&empty[st], ph ^ 1u, kWdDecodeEmpty))) {
+          *s_abort = 1;
+          ok = false;
+          break;
+        }
+        uint8_t* dst = smem + (size_t)st * a.stage_bytes;
+        // a run inside one page (P >= TS), or whole pages (stages start on page boundaries)
+        const bool one_run = P >= TS;
+        const int ncopies = one_run ? 1 : ((nt + P - 1) >> a.page_log2);
+        const int first_page = pbeg + (tok >> a.page_log2);
+        // bad page ids never reach the copy engine: the error is recorded, the stage's
+        // copies are skipped and the consumers run on what the stage held
+        bool good = true;
+        for (int j = lane; j < ncopies; j += 32) {
+          const int64_t page = a.kv_indices[first_page + j];
+          const int64_t s0 = one_run ? page * P + (tok & (P - 1)) : page * P;
+          const int rows = one_run ? nt : min(P, nt - j * P);
+          good = good && page >= 0 && s0 + rows <= a.num_slots;
+        }
+        good = __all_sync(FULL, good);
+        if (lane == 0) {
+          if (good) {
+            mbar_arrive_expect_tx(&full[st], (uint32_t)nt * a.row_bytes);
+          } else {
+            watchdog_set(kWdBadSlot);
+            mbar_arrive(&full[st]);
+          }
+        }
+        __syncwarp();
+        if (!waited) {
+          asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows of the previous kernel
+          waited = true;
+        }
+        if (good) {
+          for (int j0 = 0; j0 < ncopies; j0 += 32) {
+            // consecutive page ids are consecutive slots: one bulk copy per run of them
+            const int j = j0 + lane;
+            const int64_t page = j < ncopies ? a.kv_indices[first_page + j] : -2;
+            const int64_t prev = __shfl_up_sync(FULL, page, 1);
+            const bool head = j < ncopies && (lane == 0 || page != prev + 1);
+            const uint32_t heads = __ballot_sync(FULL, head);
+            if (head) {
+              const uint32_t above = lane == 31 ? 0u : (heads >> (lane + 1)) << (lane + 1);
+              const int end = j0 + (above ? __ffs((int)above) - 1 : min(32, ncopies - j0));
+              const int rows = one_run ? nt : min(end * P, nt) - j * P;
+              const int64_t s0 = one_run ? page * P + (tok & (P - 1)) : page * P;
+              bulk_g2s(dst + (size_t)j * P * rowB, pool + s0 * rowB, (uint32_t)rows * a.row_bytes, &full[st], pol);
+            }
+          }
+        }
+        __syncwarp();
+        ++ctr;
+      }
+    }
+    // never leave while our own copies may still be landing
+    const int first = ctr > a.NSTAGE ? ctr - a.NSTAGE : 0;
+    for (int i = first; i < ctr; ++i) mbar_wait(&full[i % a.NSTAGE], (uint32_t)(i / a.NSTAGE) & 1u, kWdDecodeDrain);
+    return;
+  }
+
+  // -------------------------------------------------------------- consumers
+  const int h = warp / a.WPH;
+  const int sub = warp - h * a.WPH;
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t code_off = fp4_code_off(h, D), scale_off = fp4_scale_off(h, a.Hkv, D);
+  float* cbuf = reinterpret_cast<float*>(smem + L.cbuf);
+  const T* qbase = reinterpret_cast<const T*>(a.q);
+  int ctr = 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // q, the workspace and out follow the previous kernel
+  for (int i = 0; i < seg1 - seg0; ++i) {
+    const int si = decode_seg_at(a, seg0, seg1, last_first, i);
+    int b, pbeg, ntok, slot;
+    decode_get_seg(a, si, b, pbeg, ntok, slot);
+    if (!decode_seg_ok(a, b, slot)) {
+      if (threadIdx.x == 0) watchdog_set(kWdBadPlan);
+      continue;
+    }
+    // ---- Q^T: head column g, features [t D/4, (t+1) D/4); zero columns past the group
+    uint32_t qf[SPLIT][KS][2];
+    float qs[2];
+    {
+      float qv[D / 4];
+      if (g < G) {
+        load_vec<T, D / 4>(qbase + ((size_t)b * a.Hq + h * G + g) * D + t * (D / 4), qv);
+      } else {
+#pragma unroll
+        for (int e = 0; e < D / 4; ++e) qv[e] = 0.f;
+      }
+      float amax = 0.f;
+#pragma unroll
+      for (int e = 0; e < D / 4; ++e) amax = fmaxf(amax, fabsf(qv[e]));
+      amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 2));
+      float f, inv;
+      fp4_row_factor(amax, f, inv);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float e0 = qv[4 * k + 2 * j] * f, e1 = qv[4 * k + 2 * j + 1] * f;
+          qf[0][k][j] = pack_h2(e0, e1);
+          if constexpr (SPLIT == 2) {
+            const float2 r = h2_to_f2(qf[0][k][j]);
+            qf[1][k][j] = pack_h2(e0 - r.x, e1 - r.y);
+          }
+        }
+      }
+      inv *= a.qscale;
+      qs[0] = __shfl_sync(FULL, inv, 8 * t);      // column 2t
+      qs[1] = __shfl_sync(FULL, inv, 8 * t + 4);  // column 2t + 1
+    }
+    float acc[KS][4];
+#pragma unroll
+    for (int mt = 0; mt < KS; ++mt) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
+    float mref[2] = {kNegInf, kNegInf}, lsum[2] = {0.f, 0.f};
+    for (int tok = 0; tok < ntok; tok += TS) {
+      const int nt = min(TS, ntok - tok);
+      const int st = ctr % a.NSTAGE;
+      const uint32_t ph = (uint32_t)(ctr / a.NSTAGE) & 1u;
+      bool ok = __all_sync(FULL, *s_abort == 0);
+      if (ok) ok = __all_sync(FULL, mbar_wait(&full[st], ph, kWdDecodeFull));
+      if (!ok) *s_abort = 1;
+      if (ok) {
+        const uint8_t* rows = smem + (size_t)st * a.stage_bytes;
+        for (int t0 = sub * kFp4Tok; t0 < nt; t0 += a.WPH * kFp4Tok)
+          fp4_unit<D, SPLIT>(rows + (size_t)t0 * a.row_bytes, a.row_bytes, code_off, scale_off,
+                             min(kFp4Tok, nt - t0), lane, qs, qf, acc, mref, lsum);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+      ++ctr;
+    }
+    // ---- row sums over the 8 lanes of each head column
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      lsum[n] += __shfl_xor_sync(FULL, lsum[n], 4);
+      lsum[n] += __shfl_xor_sync(FULL, lsum[n], 8);
+      lsum[n] += __shfl_xor_sync(FULL, lsum[n], 16);
+    }
+    // lane (g, t) holds features [g D/8, (g+1) D/8) of head columns 2t, 2t + 1: feature
+    // 2 mt of the run in acc[mt][n], 2 mt + 1 in acc[mt][2 + n]
+    constexpr int EPL = D / 8;
+    if (a.WPH > 1) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int c = 2 * t + n;
+        if (c < G) {
+          float* mine = cbuf + ((size_t)warp * G + c) * (D + 2);
+#pragma unroll
+          for (int mt = 0; mt < KS; ++mt)
+            *reinterpret_cast<float2*>(mine + g * EPL + 2 * mt) = make_float2(acc[mt][n], acc[mt][2 + n]);
+          if (g == 0) *reinterpret_cast<float2*>(mine + D) = make_float2(mref[n], lsum[n]);
+        }
+      }
+      named_bar_sync(1, NCW * 32);
+      if (sub == 0) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int c = 2 * t + n;
+          if (c < G) {
+            float M = kNegInf, Lsum = 0.f;
+            for (int s2 = 0; s2 < a.WPH; ++s2) M = fmaxf(M, cbuf[((size_t)(warp + s2) * G + c) * (D + 2) + D]);
+#pragma unroll
+            for (int mt = 0; mt < KS; ++mt) acc[mt][n] = acc[mt][2 + n] = 0.f;
+            for (int s2 = 0; s2 < a.WPH; ++s2) {
+              const float* o = cbuf + ((size_t)(warp + s2) * G + c) * (D + 2);
+              const float w = (o[D] == kNegInf) ? 0.f : exp2f(o[D] - M);
+              Lsum += o[D + 1] * w;
+#pragma unroll
+              for (int mt = 0; mt < KS; ++mt) {
+                const float2 v = *reinterpret_cast<const float2*>(o + g * EPL + 2 * mt);
+                acc[mt][n] = fmaf(w, v.x, acc[mt][n]);
+                acc[mt][2 + n] = fmaf(w, v.y, acc[mt][2 + n]);
+              }
+            }
+            mref[n] = M;
+            lsum[n] = Lsum;
+          }
+        }
+      }
+    }
+    if (sub == 0) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int c = 2 * t + n;
+        if (c < G) {
+          const size_t row = (size_t)h * G + c;
+          float r[EPL];
+          const float f = slot < 0 ? (lsum[n] > 0.f ? v_scale / lsum[n] : 0.f) : v_scale;
+#pragma unroll
+          for (int mt = 0; mt < KS; ++mt) {
+            r[2 * mt] = acc[mt][n] * f;
+            r[2 * mt + 1] = acc[mt][2 + n] * f;
+          }
+          if (slot < 0) {
+            store_vec<T, EPL>(reinterpret_cast<T*>(a.out) + ((size_t)b * a.Hq + row) * D + g * EPL, r);
+          } else {
+            store_vec<float, EPL>(a.ws_acc + ((size_t)slot * a.Hq + row) * D + g * EPL, r);
+            if (g == 0)
+              *reinterpret_cast<float2*>(a.ws_ml + ((size_t)slot * a.Hq + row) * 2) = make_float2(mref[n], lsum[n]);
+          }
+        }
+      }
+      if (slot >= 0) __threadfence();  // publish the partial rows at GPU scope before the ticket
+    }
+    if (slot >= 0) {
+      // merge ticket of request b, as in decode_kernel
+      named_bar_sync(1, NCW * 32);
+      const int p0 = a.merge_indptr[b], p1 = a.merge_indptr[b + 1];
+      if (threadIdx.x == 0) {
+        const int prev = atomicAdd(&a.tickets[p0], 1);
+        const bool last = prev == p1 - p0 - 1;
+        if (last) a.tickets[p0] = 0;  // every partial has arrived: re-arm for the next call
+        *s_last = last ? 1 : 0;
+      }
+      named_bar_sync(1, NCW * 32);
+      if (*s_last) {
+        __threadfence();
+        decode_merge_request<T, D>(a, b, p0, p1, warp, lane);
+      }
+    } else if (a.WPH > 1) {
+      named_bar_sync(1, NCW * 32);
+    }
+  }
+}
+
+}  // namespace b2a

@@ -1,0 +1,212 @@
+// The 4-bit KV pool: its row layout, the store that quantises and scatters new
+// k/v rows, and the load that reads rows back as plain values.
+//
+// Format. A head row of D features is cut into blocks of 16. A block keeps one
+// e4m3 scale s = rne_e4m3(min(max|x| / 6, 448)) and sixteen e2m1 codes
+// rne_e2m1(x / s), clipped to +-6: a value is code * s, 4.5 bits per feature.
+// The pool holds finite values only: a NaN is stored as 0 and does not count
+// for the maximum, an infinity is clipped to the block's largest value
+// (6 * 448). code * s has at most 2 + 4 significant bits and an exponent in
+// [-10, 11], so it is exact in fp16 and in bf16, and attention over the pool
+// multiplies exactly what load returns.
+//
+// Exactness of the codes: x, max|x| and s are floats, and a border between two
+// codes (or two scales) times s (times 6) has at most 7 significant bits, so a
+// quotient on a border is exact and one that is not keeps its side when it is
+// rounded to fp32. Codes are therefore those of the exact quotient, and any
+// correct implementation agrees bit for bit.
+//
+// Row of one token slot (fp4_row_bytes, a multiple of 16):
+//   [K codes D/2 | V codes D/2] for each kv head, then
+//   [K scales D/16 | V scales D/16] for each kv head, then padding.
+// Feature 2i of a row sits in the low nibble of byte i. All heads of a token
+// are one run, a page is one run of page_size rows: one bulk copy brings K and
+// V, codes and scales. A row that would be a multiple of 128 bytes gets 16 more
+// (8 heads x 128: 1168 instead of 1152, +1.4% traffic): consumers read the
+// same offset of several rows at once, and with a pitch of 128 k bytes these
+// fall into the same shared-memory banks (8-way conflicts).
+#pragma once
+
+#include "common.cuh"
+
+namespace b2a {
+
+constexpr int kFp4Block = 16;  // features per scale
+
+__host__ __device__ inline uint32_t fp4_row_bytes(int Hkv, int D) {
+  uint32_t r = (uint32_t)Hkv * (uint32_t)(D + D / 8);
+  r = (r + 15u) & ~15u;
+  if (r % 128u == 0) r += 16u;
+  return r;
+}
+// Offsets inside a token row: codes of K (V follows after D/2), scales of K (V after D/16).
+__host__ __device__ __forceinline__ uint32_t fp4_code_off(int h, int D) { return (uint32_t)(h * D); }
+__host__ __device__ __forceinline__ uint32_t fp4_scale_off(int h, int Hkv, int D) {
+  return (uint32_t)(Hkv * D + h * (D / 8));
+}
+
+// Eight codes (one word) -> four fp16 pairs, in order. Exact.
+__device__ __forceinline__ void fp4_word_to_h2(uint32_t w, uint32_t (&r)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(w));
+}
+
+// Two e4m3 scales (low byte first) -> an fp16 pair. Exact.
+__device__ __forceinline__ uint32_t fp4_scale2_to_h2(uint32_t two_bytes) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two_bytes));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// float -> e4m3 byte, to nearest even, clipped to 448 (x >= 0, not NaN).
+__device__ __forceinline__ uint32_t f_to_e4m3(float x) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(x));
+  return r & 0xffu;
+}
+
+// Two floats -> a byte of two e2m1 codes (lo in the low nibble), nearest even, clipped to +-6.
+__device__ __forceinline__ uint32_t f2_to_e2m1(float lo, float hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0;\n\t.reg .b16 h;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %1, %2;\n\t"
+      "mov.b16 h, {b0, 0};\n\t"
+      "cvt.u32.u16 %0, h;\n\t}"
+      : "=r"(r)
+      : "f"(hi), "f"(lo));
+  return r;
+}
+
+// The sixteen values of a block (before the pool's own factor), exact.
+__device__ __forceinline__ void fp4_expand16(uint2 codes, uint32_t scale_byte, float (&x)[16]) {
+  const uint32_t sh = fp4_scale2_to_h2(scale_byte | (scale_byte << 8));
+  uint32_t r0[4], r1[4];
+  fp4_word_to_h2(codes.x, r0);
+  fp4_word_to_h2(codes.y, r1);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t lo = h2_mul(r0[j], sh), hi = h2_mul(r1[j], sh);
+    const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+    const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    x[2 * j] = f0.x;
+    x[2 * j + 1] = f0.y;
+    x[8 + 2 * j] = f1.x;
+    x[9 + 2 * j] = f1.y;
+  }
+}
+
+struct Fp4KvArgs {
+  const void* k;  // store: new rows
+  const void* v;
+  void* k_out;  // load: destinations [n, Hkv, D]
+  void* v_out;
+  int64_t k_stride, v_stride;  // elements between token rows (store)
+  const int32_t* slots;
+  uint8_t* pool;
+  int64_t num_slots;
+  int64_t n;  // token rows
+  int Hkv;
+  int nblk;  // blocks of a head row: D / 16
+  uint32_t row_bytes;
+  float k_scale, v_scale;  // powers of two: a stored value stands for code * s * scale
+};
+
+template <typename T>
+__device__ __forceinline__ void fp4_read16(const T* p, bool vec, float (&x)[16]) {
+  if (vec) {
+    load_vec<T, 16>(p, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = DT<T>::to_f(p[i]);
+  }
+}
+
+// One thread quantises one block of 16 features: 32 or 64 bytes in, 8 + 1 bytes
+// out. Bound by HBM at large T. Neighbouring threads hold neighbouring blocks of
+// a row, so reads and code writes are contiguous over a token's heads.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) fp4_store_kernel(const Fp4KvArgs a) {
+  pdl_wait_then_release();
+  const int64_t per_tok = 2ll * a.Hkv * a.nblk;
+  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= a.n * per_tok) return;
+  const int64_t t = i / per_tok;
+  const int rem = (int)(i - t * per_tok);
+  const int kind = rem >= a.Hkv * a.nblk;  // 0: k, 1: v
+  const int hb = rem - kind * a.Hkv * a.nblk;
+  const int h = hb / a.nblk, blk = hb - h * a.nblk;
+  const int D = a.nblk * kFp4Block;
+  const int64_t slot = a.slots[t];
+  if (slot < 0 || slot >= a.num_slots) {
+    watchdog_set(kWdBadSlot);
+    return;
+  }
+  const T* src = reinterpret_cast<const T*>(kind ? a.v : a.k) + t * (kind ? a.v_stride : a.k_stride) + hb * kFp4Block;
+  float x[16];
+  fp4_read16<T>(src, VEC, x);
+  const float inv_g = 1.f / (kind ? a.v_scale : a.k_scale);  // exact: a power of two
+  float amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    x[j] = (x[j] != x[j]) ? 0.f : x[j] * inv_g;
+    amax = fmaxf(amax, fabsf(x[j]));
+  }
+  const uint32_t sb = f_to_e4m3(fminf(__fdiv_rn(amax, 6.f), 448.f));
+  const uint32_t sh = fp4_scale2_to_h2(sb);
+  const float s = __half2float(__ushort_as_half((unsigned short)(sh & 0xffffu)));
+  uint32_t w[2] = {0u, 0u};
+  if (s > 0.f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      w[j >> 2] |= f2_to_e2m1(__fdiv_rn(x[2 * j], s), __fdiv_rn(x[2 * j + 1], s)) << (8 * (j & 3));
+  }
+  uint8_t* row = a.pool + (size_t)slot * a.row_bytes;
+  *reinterpret_cast<uint2*>(row + fp4_code_off(h, D) + kind * (D / 2) + blk * 8) = make_uint2(w[0], w[1]);
+  row[fp4_scale_off(h, a.Hkv, D) + kind * a.nblk + blk] = (uint8_t)sb;
+}
+
+// One thread expands one block of 16: 8 + 1 bytes in, 32 or 64 bytes out.
+template <typename T>
+__global__ void __launch_bounds__(256) fp4_load_kernel(const Fp4KvArgs a) {
+  pdl_wait_then_release();
+  const int64_t per_tok = 2ll * a.Hkv * a.nblk;
+  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= a.n * per_tok) return;
+  const int64_t t = i / per_tok;
+  const int rem = (int)(i - t * per_tok);
+  const int kind = rem >= a.Hkv * a.nblk;
+  const int hb = rem - kind * a.Hkv * a.nblk;
+  const int h = hb / a.nblk, blk = hb - h * a.nblk;
+  const int D = a.nblk * kFp4Block;
+  const int64_t slot = a.slots[t];
+  uint2 c = make_uint2(0u, 0u);  // a slot outside the pool reads as zeros
+  uint32_t sb = 0;
+  if (slot < 0 || slot >= a.num_slots) {
+    watchdog_set(kWdBadSlot);
+  } else {
+    const uint8_t* row = a.pool + (size_t)slot * a.row_bytes;
+    c = *reinterpret_cast<const uint2*>(row + fp4_code_off(h, D) + kind * (D / 2) + blk * 8);
+    sb = row[fp4_scale_off(h, a.Hkv, D) + kind * a.nblk + blk];
+  }
+  const float g = kind ? a.v_scale : a.k_scale;
+  float x[16];
+  fp4_expand16(c, sb, x);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) x[j] *= g;
+  T* dst = reinterpret_cast<T*>(kind ? a.v_out : a.k_out) + (t * a.Hkv * a.nblk + hb) * kFp4Block;
+  store_vec<T, 16>(dst, x);
+}
+
+}  // namespace b2a

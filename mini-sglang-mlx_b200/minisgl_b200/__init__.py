@@ -14,7 +14,7 @@ from .attention import (
 )
 from .config import ModelConfig, RotaryConfig
 from .core import Batch, Context, Req, get_global_ctx, set_global_ctx
-from .kvcache import MHAKVCache
+from .kvcache import FP4KVCache, MHAKVCache
 from .layers import AttentionLayer, RotaryEmbedding
 
 __all__ = [
@@ -23,6 +23,7 @@ __all__ = [
     "BaseAttnBackend",
     "Batch",
     "Context",
+    "FP4KVCache",
     "MHAKVCache",
     "ModelConfig",
     "Req",

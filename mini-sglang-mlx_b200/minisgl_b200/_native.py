@@ -98,6 +98,29 @@ SIGNATURES = {
     ),
     "b2a_swiglu": (c_int, [_P, c_int64, _P, c_int64, c_int, c_int, _P]),
     "b2a_rmsnorm": (c_int, [_P, c_int64, c_int64, _P, c_int64, _P, c_float, c_int, _P, c_int, _P]),
+    "b2a_fp4_row_bytes": (c_size_t, [c_int, c_int]),
+    "b2a_fp4_store_kv": (
+        c_int,
+        [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64, c_int, c_int, c_float, c_float, c_int, _P],
+    ),
+    "b2a_fp4_load_kv": (c_int, [_P, c_int64, _P, c_int64, c_int, c_int, c_float, c_float, _P, _P, c_int, _P]),
+    "b2a_fp4_decode_num_ctas": (c_int, [c_int, c_int, c_int, c_int, ctypes.POINTER(c_int)]),
+    "b2a_fp4_decode": (
+        c_int,
+        [_P, _P, c_int64, _P, c_int, _P, _P, c_int, _P, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_float,
+         _P, c_size_t, _P, c_int, _P],
+    ),
+    "b2a_fp4_extend_tile_q": (c_int, [c_int, c_int, c_int, c_int, ctypes.POINTER(c_int)]),
+    "b2a_fp4_extend": (
+        c_int,
+        [_P, _P, c_int64, _P, _P, _P, _P, c_int, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float,
+         c_float, _P, c_int, _P],
+    ),
+    "b2a_extend_metadata": (
+        c_int,
+        [_P, c_int64, c_int64, _P, _P, _P, c_int, c_int, c_int, _P, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P,
+         c_int, _P, _P],
+    ),
     "b2a_proj": (c_int, [_P, c_int64, c_int, c_int, _P, c_int, _P, c_float, _P, c_int64, _P, c_int64, c_int, c_int,
                          _P]),
 }
@@ -170,6 +193,12 @@ def decode_plan(kv_indptr: np.ndarray, kv_last_page_len: np.ndarray | None, page
 def extend_tile_q(Hq: int, Hkv: int, D: int, dtype_code: int, page_size: int) -> int:
     t = c_int(0)
     call("b2a_extend_tile_q", Hq, Hkv, D, dtype_code, page_size, ctypes.byref(t))
+    return t.value
+
+
+def fp4_extend_tile_q(Hq: int, Hkv: int, D: int, dtype_code: int) -> int:
+    t = c_int(0)
+    call("b2a_fp4_extend_tile_q", Hq, Hkv, D, dtype_code, ctypes.byref(t))
     return t.value
 
 

@@ -24,6 +24,7 @@ import torch
 
 from .. import _native as nat
 from ..core import get_global_ctx
+from ..kvcache.fp4 import FP4KVCache, on_device
 from ..kvcache.pool import current_stream_ptr, dtype_code
 from .base import CHECK_METADATA, BaseAttnBackend, PinnedStager, paged_kv_indices
 
@@ -62,6 +63,12 @@ class B200PrefillMetadata:
     # into a staging pool first (b2a_pack_kv) and their starts point there (>= num_slots)
     pack: "PackPlan | None" = None
     group_starts: bool = False
+    # set by alloc_extend_metadata (device-built metadata): the new tokens' positions and pool
+    # slots, and int32 [2] new tokens, tiles; q_offsets is then empty
+    positions: torch.Tensor | None = None
+    out_loc: torch.Tensor | None = None
+    counts: torch.Tensor | None = None
+    tile_q: int = 0
 
 
 @dataclass
@@ -86,6 +93,8 @@ class B200AttnBackend(BaseAttnBackend):
         if not torch.cuda.is_available():
             raise RuntimeError("the b200 attention backend needs a CUDA device")
         self.device = kv_cache.device
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self.Hq = config.num_qo_heads
         self.Hkv = config.num_kv_heads
         self.D = config.head_dim
@@ -94,15 +103,28 @@ class B200AttnBackend(BaseAttnBackend):
         self._stager = PinnedStager()
         self._workspace = torch.empty(0, dtype=torch.uint8, device=self.device)
         self._stage: tuple | None = None  # packed K/V staging pools for small-page prefill
+        self.fp4 = isinstance(kv_cache, FP4KVCache)  # the pool holds 4-bit rows (kvcache/fp4.py)
         n = nat.ctypes.c_int(0)
         with torch.cuda.device(self.device):
-            nat.call("b2a_decode_num_ctas", self.Hq, self.Hkv, self.D, self.dtype_code, nat.ctypes.byref(n))
+            nat.call("b2a_fp4_decode_num_ctas" if self.fp4 else "b2a_decode_num_ctas", self.Hq, self.Hkv, self.D, self.dtype_code, nat.ctypes.byref(n))
         self.num_ctas = n.value
 
     # ------------------------------------------------------------ helpers
     @property
     def page_size(self) -> int:
         return self._page_size if self._page_size is not None else _page_size()
+
+    def _query(self, q: torch.Tensor) -> torch.Tensor:
+        """q as the kernels read it: contiguous; over a 4-bit pool also of the cache's dtype and device."""
+        if self.fp4 and (q.dtype != self.kv_cache.dtype or q.device != self.device):
+            raise ValueError(f"attention over the 4-bit pool: q must be {self.kv_cache.dtype} on {self.device}, got "
+                             f"{q.dtype} on {q.device}")
+        return q.contiguous()
+
+    def _tile_q(self, page_size: int) -> int:
+        if self.fp4:
+            return nat.fp4_extend_tile_q(self.Hq, self.Hkv, self.D, self.dtype_code)
+        return nat.extend_tile_q(self.Hq, self.Hkv, self.D, self.dtype_code, page_size)
 
     def _workspace_for(self, nbytes: int) -> torch.Tensor:
         # zero-filled once: the merge counters at its start must be zero before the
@@ -208,11 +230,22 @@ class B200AttnBackend(BaseAttnBackend):
     def forward_decode(self, q: torch.Tensor, layer_id: int, meta: B200DecodeMetadata) -> torch.Tensor:
         B = meta.batch_size
         assert q.shape == (B, self.Hq, self.D), q.shape
-        q = q.contiguous()
+        q = self._query(q)
         out = torch.empty_like(q)
         ws_bytes = nat.decode_workspace_bytes(meta.n_partials, self.Hq, self.D)
         ws = meta.workspace if meta.workspace is not None else self._workspace_for(ws_bytes)
         assert ws.numel() >= ws_bytes
+        if self.fp4:
+            kv = self.kv_cache
+            with on_device(self.device):
+                nat.call(
+                    "b2a_fp4_decode", q.data_ptr(), kv.rows(layer_id).data_ptr(), kv.num_tokens,
+                    meta.kv_indices.data_ptr(), meta.page_size, meta.cta_indptr.data_ptr(), meta.segs.data_ptr(),
+                    meta.num_ctas, meta.merge_indptr.data_ptr(), meta.n_partials, B, self.Hq, self.Hkv, self.D,
+                    float(self.scale), kv.k_scale, kv.v_scale, ws.data_ptr(), ws.numel(), out.data_ptr(),
+                    self.dtype_code, current_stream_ptr(self.device),
+                )
+            return out
         nat.call(
             "b2a_decode", q.data_ptr(), self.kv_cache.k_cache(layer_id).data_ptr(),
             self.kv_cache.v_cache(layer_id).data_ptr(), self.kv_cache.num_tokens, meta.kv_indices.data_ptr(),
@@ -236,9 +269,9 @@ class B200AttnBackend(BaseAttnBackend):
         qo_indptr = np.zeros(len(extend) + 1, np.int32)
         np.cumsum(extend, out=qo_indptr[1:])
         kv_indptr, kv_indices, lpl = paged_kv_indices(self.page_table, rows, lens, P, check=CHECK_METADATA)
-        tile_q = nat.extend_tile_q(self.Hq, self.Hkv, self.D, self.dtype_code, P)
+        tile_q = self._tile_q(P)
         if P < self.PACK_PAGE:
-            tile16 = nat.extend_tile_q(self.Hq, self.Hkv, self.D, self.dtype_code, self.PACK_PAGE)
+            tile16 = self._tile_q(self.PACK_PAGE)
             if tile16 != tile_q:  # the tensor-core kernel takes this shape in groups of 16 keys
                 return self._grouped_extend_metadata(qo_indptr, np.asarray(lens, dtype=np.int64), kv_indptr,
                                                      kv_indices, P, tile16)
@@ -252,6 +285,66 @@ class B200AttnBackend(BaseAttnBackend):
         )
 
     PACK_PAGE = 16
+
+    # ------------------------------------------------------------ prefill metadata built on the device
+    def alloc_extend_metadata(self, batch_size: int, total_q: int, total_pages: int,
+                              tile_q: int | None = None) -> B200PrefillMetadata:
+        """Prefill metadata of ``batch_size`` requests for ``build_extend_metadata_device`` to fill.
+
+        ``total_q`` new tokens and ``total_pages`` pages in all: what the batch needs, or the
+        capacity of a batch whose lengths are known on the device only (a captured step). A batch
+        that needs less leaves the tails of ``positions``, ``out_loc`` and ``kv_indices`` as they
+        were, and empty tiles at the end of ``work``. ``tile_q`` defaults to the tile of this
+        backend's extend kernel.
+        """
+        P = self.page_size
+        if tile_q is None:
+            tile_q = self._tile_q(P)
+            if P < self.PACK_PAGE and tile_q != self._tile_q(self.PACK_PAGE):
+                raise ValueError(f"alloc_extend_metadata: page size {P} needs the host-built key groups "
+                                 "(extend_metadata_from_lens)")
+        if batch_size < 1 or total_q < 0 or total_pages < 0 or tile_q < 1:
+            raise ValueError(f"alloc_extend_metadata: batch {batch_size}, {total_q} tokens, {total_pages} pages, "
+                             f"tile {tile_q}")
+        n_work = min(batch_size, total_q) + total_q // tile_q
+        sizes = [batch_size + 1, total_q, total_q, batch_size, batch_size + 1, total_pages, batch_size, 4 * n_work, 2]
+        # one allocation, every array on a 64-byte boundary (work is written as int4)
+        starts = np.cumsum([0] + [(n + 15) // 16 * 16 for n in sizes])
+        buf = torch.zeros(int(starts[-1]), dtype=torch.int32, device=self.device)
+        qo, pos, loc, last, kv, idx, lpl, work, counts = (buf[int(o): int(o) + n] for o, n in zip(starts, sizes))
+        return B200PrefillMetadata(
+            last_indices=last, q_offsets=[], qo_indptr=qo, kv_indptr=kv, kv_indices=idx, kv_last_page_len=lpl,
+            work=work.view(-1, 4), n_work=n_work, total_q=total_q, page_size=P, positions=pos, out_loc=loc,
+            counts=counts, tile_q=tile_q)
+
+    def build_extend_metadata_device(self, meta: B200PrefillMetadata, page_table: torch.Tensor, rows: torch.Tensor,
+                                     cached: torch.Tensor, lens: torch.Tensor) -> None:
+        """Fill ``meta`` (from ``alloc_extend_metadata``) on the device (b2a_extend_metadata).
+
+        ``page_table`` is a device int32 copy of the engine's page table; ``rows``, ``cached`` and
+        ``lens`` are device int32 ``[B]``: page-table row, tokens already in the pool and all tokens
+        of every request. One launch, stream-ordered, capturable in a CUDA graph. The values equal
+        ``extend_metadata_from_lens``'s and ``batch_positions_out_loc``'s for the same lengths.
+        """
+        B = meta.qo_indptr.numel() - 1
+        if meta.counts is None:
+            raise ValueError("build_extend_metadata_device: metadata not from alloc_extend_metadata")
+        if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous() \
+                or page_table.device != self.device:
+            raise ValueError(f"page_table must be contiguous int32 [rows, tokens] on {self.device}")
+        for name, t in (("rows", rows), ("cached", cached), ("lens", lens)):
+            if t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous() or t.device != self.device:
+                raise ValueError(f"{name} must be contiguous int32 [{B}] on {self.device}, got {t.dtype} "
+                                 f"{tuple(t.shape)} on {t.device}")
+        with on_device(self.device):
+            nat.call(
+                "b2a_extend_metadata", page_table.data_ptr(), page_table.shape[0], page_table.shape[1],
+                rows.data_ptr(), cached.data_ptr(), lens.data_ptr(), B, meta.page_size, meta.tile_q,
+                meta.qo_indptr.data_ptr(), meta.positions.data_ptr(), meta.out_loc.data_ptr(), meta.positions.numel(),
+                meta.last_indices.data_ptr(), meta.kv_indptr.data_ptr(), meta.kv_indices.data_ptr(),
+                meta.kv_indices.numel(), meta.kv_last_page_len.data_ptr(), meta.work.data_ptr(), meta.n_work,
+                meta.counts.data_ptr(), current_stream_ptr(self.device),
+            )
 
     def _grouped_extend_metadata(self, qo_indptr, lens, src_indptr, src_indices, P, tile_q) -> B200PrefillMetadata:
         """Extend metadata for a pool whose page size is below 16 (b2a_extend_groups): the
@@ -289,9 +382,20 @@ class B200AttnBackend(BaseAttnBackend):
     def _forward_prefill(self, q, k, v, layer_id: int, meta: B200PrefillMetadata) -> torch.Tensor:
         T = meta.total_q
         assert q.shape == (T, self.Hq, self.D), q.shape
-        q = q.contiguous()
+        q = self._query(q)
         out = torch.empty_like(q)
-        B = len(meta.q_offsets) - 1
+        B = meta.qo_indptr.numel() - 1
+        if self.fp4:
+            kv = self.kv_cache
+            with on_device(self.device):
+                nat.call(
+                    "b2a_fp4_extend", q.data_ptr(), kv.rows(layer_id).data_ptr(), kv.num_tokens,
+                    meta.qo_indptr.data_ptr(), meta.kv_indptr.data_ptr(), meta.kv_indices.data_ptr(),
+                    meta.kv_last_page_len.data_ptr(), meta.page_size, meta.work.data_ptr(), meta.n_work, T, B, self.Hq,
+                    self.Hkv, self.D, float(self.scale), kv.k_scale, kv.v_scale, out.data_ptr(), self.dtype_code,
+                    current_stream_ptr(self.device),
+                )
+            return out
         k_pool, v_pool = self.kv_cache.k_cache(layer_id), self.kv_cache.v_cache(layer_id)
         num_slots = self.kv_cache.num_tokens
         if meta.group_starts:

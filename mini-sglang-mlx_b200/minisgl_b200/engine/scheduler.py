@@ -31,7 +31,7 @@ import torch
 from ..attention import create_attention_backend, page_table_scatter
 from ..attention.base import PinnedStager
 from ..core import Batch, Context, Req, SamplingParams, batch_positions_out_loc, set_global_ctx
-from ..kvcache import MHAKVCache
+from ..kvcache import FP4KVCache, MHAKVCache
 from .graph import DecodeGraphs
 from .managers import CacheManager, ChunkedReq, DecodeManager, PrefillManager, TableManager
 from .model import Qwen3Model, Qwen3Spec
@@ -61,6 +61,9 @@ class EngineConfig:
     # bf16 steps of <= 32 tokens run the layers' projections as b2a_proj launches with the
     # norms, residual adds and SwiGLU fused in (False: cuBLAS + separate kernels throughout)
     fused_proj: bool = True
+    # "auto": the KV pool holds `dtype`; "fp4": 4-bit rows (FP4KVCache), 3.5 times the tokens in
+    # the bytes of a bf16 pool
+    kv_cache_dtype: str = "auto"
     seed: int = 42
 
 
@@ -74,8 +77,10 @@ class Engine:
         self.model.fused_proj = self.model.fused_proj and cfg.fused_proj
         P = cfg.page_size
         self.num_tokens = cfg.num_tokens // P * P
-        self.kv_cache = MHAKVCache(a.num_layers, self.num_tokens, a.num_kv_heads, a.head_dim, self.dtype,
-                                   device=self.device)
+        if cfg.kv_cache_dtype not in ("auto", "fp4"):
+            raise ValueError(f"Unknown kv_cache_dtype {cfg.kv_cache_dtype!r}: ['auto', 'fp4']")
+        pool = FP4KVCache if cfg.kv_cache_dtype == "fp4" else MHAKVCache
+        self.kv_cache = pool(a.num_layers, self.num_tokens, a.num_kv_heads, a.head_dim, self.dtype, device=self.device)
         self.max_seq_len = cfg.max_seq_len or min(a.rotary_config.max_position, self.num_tokens)
         # the pool's last page and the page table's last row are reserved for padded
         # CUDA-graph batches: a pad request is one token at the pad slot

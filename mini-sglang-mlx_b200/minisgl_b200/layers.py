@@ -25,6 +25,7 @@ import torch
 from . import _native as nat
 from .config import RotaryConfig
 from .core import get_global_ctx
+from .kvcache.fp4 import FP4KVCache, on_device
 from .kvcache.pool import current_stream_ptr, dtype_code
 
 
@@ -108,6 +109,18 @@ class RotaryEmbedding:
         for w in (q_norm_w, k_norm_w):
             assert w is None or (w.shape == (D,) and w.dtype == q.dtype and w.is_contiguous())
         assert q_out is None or (q_out.shape == q.shape and q_out.is_contiguous() and q_out.dtype == q.dtype)
+        if isinstance(kv_cache, FP4KVCache):
+            # norm and rotation as for a 16-bit pool, k in place; then k and v are quantised into their slots
+            with on_device(kv_cache.device):
+                nat.call(
+                    "b2a_qknorm_rope_store", q.data_ptr(), q.stride(0), None if q_out is None else q_out.data_ptr(),
+                    k.data_ptr(), k.stride(0), None, 0, None if q_norm_w is None else q_norm_w.data_ptr(),
+                    None if k_norm_w is None else k_norm_w.data_ptr(), float(eps), positions.data_ptr(), None, None,
+                    None, 0, self.inv_freq.data_ptr(), float(self.scale), self.dims, T, Hq, Hkv, D,
+                    dtype_code(q.dtype), current_stream_ptr(q.device),
+                )
+            kv_cache.store_kv(k, v, out_loc, layer_id)
+            return
         nat.call(
             "b2a_qknorm_rope_store", q.data_ptr(), q.stride(0), None if q_out is None else q_out.data_ptr(),
             k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
