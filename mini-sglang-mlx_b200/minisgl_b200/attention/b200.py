@@ -69,6 +69,9 @@ class B200PrefillMetadata:
     out_loc: torch.Tensor | None = None
     counts: torch.Tensor | None = None
     tile_q: int = 0
+    # 4-bit pool: runs the keys of a work item are cut into, and the workspace of their partial rows
+    n_split: int = 1
+    workspace: torch.Tensor | None = None
 
 
 @dataclass
@@ -266,6 +269,7 @@ class B200AttnBackend(BaseAttnBackend):
     def extend_metadata_from_lens(self, rows: np.ndarray, lens: np.ndarray,
                                   extend: np.ndarray) -> B200PrefillMetadata:
         P = self.page_size
+        lens = np.asarray(lens)
         qo_indptr = np.zeros(len(extend) + 1, np.int32)
         np.cumsum(extend, out=qo_indptr[1:])
         kv_indptr, kv_indices, lpl = paged_kv_indices(self.page_table, rows, lens, P, check=CHECK_METADATA)
@@ -278,11 +282,24 @@ class B200AttnBackend(BaseAttnBackend):
         work = nat.extend_plan(qo_indptr, kv_indptr, lpl, P, tile_q)
         last_indices = (qo_indptr[1:] - 1).astype(np.int32)
         dev = self._stager.upload([last_indices, qo_indptr, kv_indptr, kv_indices, lpl, work], self.device)
-        return B200PrefillMetadata(
+        meta = B200PrefillMetadata(
             last_indices=dev[0], q_offsets=qo_indptr.tolist(), qo_indptr=dev[1], kv_indptr=dev[2],
             kv_indices=dev[3], kv_last_page_len=dev[4], work=dev[5].view(-1, 4), n_work=int(work.shape[0]),
             total_q=int(qo_indptr[-1]), page_size=P,
         )
+        self._split_extend(meta, int(lens.max(initial=0)))
+        return meta
+
+    def _split_extend(self, meta: B200PrefillMetadata, max_kv_len: int) -> None:
+        """Cut the keys of few work items into runs (4-bit pool): n_split and the batch's own workspace."""
+        if not self.fp4:
+            return
+        with on_device(self.device):
+            meta.n_split = nat.fp4_extend_splits(meta.n_work, max_kv_len, self.Hq, self.Hkv, self.D, self.dtype_code)
+            nbytes = int(nat.LIB.b2a_fp4_extend_workspace_bytes(meta.n_work, meta.n_split, self.Hkv, self.D))
+            if nbytes:
+                meta.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+                meta.workspace[: 4 * meta.n_work * self.Hkv].zero_()  # the merge counters at its start
 
     PACK_PAGE = 16
 
@@ -312,10 +329,12 @@ class B200AttnBackend(BaseAttnBackend):
         starts = np.cumsum([0] + [(n + 15) // 16 * 16 for n in sizes])
         buf = torch.zeros(int(starts[-1]), dtype=torch.int32, device=self.device)
         qo, pos, loc, last, kv, idx, lpl, work, counts = (buf[int(o): int(o) + n] for o, n in zip(starts, sizes))
-        return B200PrefillMetadata(
+        meta = B200PrefillMetadata(
             last_indices=last, q_offsets=[], qo_indptr=qo, kv_indptr=kv, kv_indices=idx, kv_last_page_len=lpl,
             work=work.view(-1, 4), n_work=n_work, total_q=total_q, page_size=P, positions=pos, out_loc=loc,
             counts=counts, tile_q=tile_q)
+        self._split_extend(meta, min(total_pages * P, self.page_table.shape[1]))
+        return meta
 
     def build_extend_metadata_device(self, meta: B200PrefillMetadata, page_table: torch.Tensor, rows: torch.Tensor,
                                      cached: torch.Tensor, lens: torch.Tensor) -> None:
@@ -391,8 +410,10 @@ class B200AttnBackend(BaseAttnBackend):
                 nat.call(
                     "b2a_fp4_extend", q.data_ptr(), kv.rows(layer_id).data_ptr(), kv.num_tokens,
                     meta.qo_indptr.data_ptr(), meta.kv_indptr.data_ptr(), meta.kv_indices.data_ptr(),
-                    meta.kv_last_page_len.data_ptr(), meta.page_size, meta.work.data_ptr(), meta.n_work, T, B, self.Hq,
-                    self.Hkv, self.D, float(self.scale), kv.k_scale, kv.v_scale, out.data_ptr(), self.dtype_code,
+                    meta.kv_last_page_len.data_ptr(), meta.page_size, meta.work.data_ptr(), meta.n_work, meta.n_split,
+                    T, B, self.Hq, self.Hkv, self.D, float(self.scale), kv.k_scale, kv.v_scale,
+                    None if meta.workspace is None else meta.workspace.data_ptr(),
+                    0 if meta.workspace is None else meta.workspace.numel(), out.data_ptr(), self.dtype_code,
                     current_stream_ptr(self.device),
                 )
             return out
