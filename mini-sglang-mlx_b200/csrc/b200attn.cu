@@ -1096,12 +1096,11 @@ int fp4_decode_config(int Hq, int Hkv, int D, DecodeCfg& c) {
     return fail(B2A_ERR_UNSUPPORTED, "fp4 decode supports Hkv in {1, 2, 4, 8, 16}, got %d", Hkv);
   if (G > 8) return fail(B2A_ERR_UNSUPPORTED, "fp4 decode: GQA group %d (at most 8)", G);
   c.row_bytes = b2a::fp4_row_bytes(Hkv, D);
-  // 16 consumer warps; 8 at head_dim 256, whose accumulators need more than the ~118
-  // registers 17 warps leave a thread (16 kv heads still take a warp each)
-  c.NCW = (D == 256 && Hkv < 16) ? 8 : 16;
+  // 8 consumer warps, 16 for 16 kv heads (a warp serves one head)
+  c.NCW = Hkv == 16 ? 16 : 8;
   c.WPH = c.NCW / Hkv;
-  // a stage holds a unit of 16 tokens for every warp, more while it stays near 40 KB
-  c.TS = b2a::kFp4Tok * c.WPH;
+  // a stage holds what every warp takes at a time, more while it stays near 40 KB
+  c.TS = 16 * b2a::fp4_units_of(c.NCW) * c.WPH;
   while (2u * c.TS * c.row_bytes <= 40960u) c.TS *= 2;
   c.stage_bytes = (uint32_t)c.TS * c.row_bytes;
   const size_t fixed = b2a::fp4_decode_smem(0, c.stage_bytes, c.NCW, c.WPH, G, D).total + 6 * 16;
@@ -1125,7 +1124,7 @@ template <typename T, int D, int NCW>
 int fp4_decode_launch(const b2a::DecodeArgs& a, const DecodeCfg& c, float v_scale, int grid, cudaStream_t st) {
   auto kern = b2a::decode_fp4_kernel<T, D, NCW>;
   if (int rc = ensure_smem((const void*)kern, c.smem, "fp4_decode")) return rc;
-  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3((NCW + 1) * 32), c.smem, st, a, v_scale);
+  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3((NCW + 4) * 32), c.smem, st, a, v_scale);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(B2A_ERR_CUDA, "decode_fp4_kernel: %s", cudaGetErrorString(e));
@@ -1285,9 +1284,11 @@ int b2a_fp4_decode(const void* q, const void* pool, int64_t num_slots, const int
     using Tt = decltype(tag);
     switch (D) {
       case 64:
-        return fp4_decode_launch<Tt, 64, 16>(a, c, v_scale, num_ctas, st);
+        return c.NCW == 16 ? fp4_decode_launch<Tt, 64, 16>(a, c, v_scale, num_ctas, st)
+                           : fp4_decode_launch<Tt, 64, 8>(a, c, v_scale, num_ctas, st);
       case 128:
-        return fp4_decode_launch<Tt, 128, 16>(a, c, v_scale, num_ctas, st);
+        return c.NCW == 16 ? fp4_decode_launch<Tt, 128, 16>(a, c, v_scale, num_ctas, st)
+                           : fp4_decode_launch<Tt, 128, 8>(a, c, v_scale, num_ctas, st);
       default:
         return c.NCW == 16 ? fp4_decode_launch<Tt, 256, 16>(a, c, v_scale, num_ctas, st)
                            : fp4_decode_launch<Tt, 256, 8>(a, c, v_scale, num_ctas, st);

@@ -9,7 +9,7 @@
 // What bounds it. A cached value is 0.56 bytes, so at HBM rate an SM receives
 // about 40 values per clock (1.13 bytes and 2 G multiply-adds per K/V pair):
 // expanding and multiplying them has to cost less than a clock per 40 values.
-// One warp takes units of 16 tokens x one kv head:
+// One warp takes one or two units of 16 tokens x one kv head at a time; a unit is
 //   S^T [16 tokens x 8 head columns] = K [16 x D] . Q^T      (D/16 MMAs)
 //   O^T [D x 8]                     += V^T [D x 16] . P^T    (D/16 MMAs)
 // with mma.sync m16n8k16, fp16 in, fp32 accumulate. The codes become MMA
@@ -37,7 +37,8 @@
 
 namespace b2a {
 
-constexpr int kFp4Tok = 16;  // tokens of a unit
+// units of 16 tokens a warp takes at a time
+__host__ __device__ constexpr int fp4_units_of(int NCW) { return NCW == 16 ? 1 : 2; }
 
 struct Fp4DecodeSmem {
   uint32_t bars, cbuf, abort_flag, last_flag, total;
@@ -62,7 +63,7 @@ __host__ __device__ inline Fp4DecodeSmem fp4_decode_smem(int NSTAGE, uint32_t st
 // D += A (16x16 fp16, row) . B (16x8 fp16, col), fp32 accumulate.
 __device__ __forceinline__ void mma_16816_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                               uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -107,55 +108,76 @@ __device__ __forceinline__ void fp4_lds(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
-// One unit. row0: shared address of token 0's row; nt of its 16 tokens are real.
-// qf[p]: part p of Q^T (features of this lane's quarter, head column g).
-template <int D, int SPLIT>
-__device__ __forceinline__ void fp4_unit(const uint8_t* row0, uint32_t pitch, uint32_t code_off, uint32_t scale_off,
-                                         int nt, int lane, const float (&qs)[2], const uint32_t (&qf)[SPLIT][D / 16][2],
-                                         float (&acc)[D / 16][4], float (&mref)[2], float (&lsum)[2]) {
+// N consecutive scale bytes, each as an fp16 pair of twice the same value.
+template <int N>
+__device__ __forceinline__ void fp4_scales(const uint8_t* p, uint32_t (&s)[N]) {
+  if constexpr (N == 1) {
+    const uint32_t b = *p;
+    s[0] = fp4_scale2_to_h2(b | (b << 8));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint32_t h = fp4_scale2_to_h2(*reinterpret_cast<const uint16_t*>(p + i));
+      s[i] = __byte_perm(h, 0, 0x1010);
+      s[i + 1] = __byte_perm(h, 0, 0x3232);
+    }
+  }
+}
+
+// NU units of one head, their softmax step taken together. row0: shared address of token 0's
+// row; with PART only nt of the 16 NU tokens are real. qf[p]: part p of Q^T (features of this
+// lane's quarter, head column g).
+template <int D, int SPLIT, int NU, bool PART>
+__device__ __forceinline__ void fp4_units(const uint8_t* row0, uint32_t pitch, uint32_t code_off, uint32_t scale_off,
+                                          int nt, int lane, const float (&qs)[2],
+                                          const uint32_t (&qf)[SPLIT][D / 16][2], float (&acc)[D / 16][4],
+                                          float (&mref)[2], float (&lsum)[2]) {
   constexpr unsigned FULL = 0xffffffffu;
   constexpr int KS = D / 16;  // MMAs of a product
   const int g = lane >> 2, t = lane & 3;
-  // ---- S^T: rows g and g + 8, features [t D/4, (t+1) D/4)
-  float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-  {
-    const uint8_t* ra = row0 + (uint32_t)g * pitch;
-    const uint8_t* rb = ra + 8u * pitch;
+  // ---- S^T: rows g and g + 8 of each unit, features [t D/4, (t+1) D/4)
+  // x[u][0]: (token g, column 2t) [1]: (g, 2t+1) [2]: (g+8, 2t) [3]: (g+8, 2t+1)
+  float x[NU][4];
+  const uint8_t* krow = row0 + (uint32_t)g * pitch + code_off + t * (D / 8);
+  const uint8_t* srow = row0 + (uint32_t)g * pitch + scale_off + t * (D / 64);
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
     uint32_t wa[D / 32], wb[D / 32];
-    fp4_lds<D / 32>(ra + code_off + t * (D / 8), wa);
-    fp4_lds<D / 32>(rb + code_off + t * (D / 8), wb);
+    fp4_lds<D / 32>(krow + (16u * u) * pitch, wa);
+    fp4_lds<D / 32>(krow + (16u * u + 8u) * pitch, wb);
+    uint32_t sca[D / 64], scb[D / 64];  // a block's scale, twice
+    fp4_scales<D / 64>(srow + (16u * u) * pitch, sca);
+    fp4_scales<D / 64>(srow + (16u * u + 8u) * pitch, scb);
 #pragma unroll
-    for (int q = 0; q < D / 64; ++q) {  // one block of 16 features: 2 words, 4 MMAs
-      const uint32_t sa8 = ra[scale_off + t * (D / 64) + q], sb8 = rb[scale_off + t * (D / 64) + q];
-      const uint32_t sa = fp4_scale2_to_h2(sa8 | (sa8 << 8)), sb = fp4_scale2_to_h2(sb8 | (sb8 << 8));
+    for (int w = 0; w < D / 32; ++w) {  // eight features of both rows: two MMAs
+      uint32_t xa[4], xb[4];
+      fp4_word_to_h2(wa[w], xa);
+      fp4_word_to_h2(wb[w], xb);
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        uint32_t xa[4], xb[4];
-        fp4_word_to_h2(wa[2 * q + w], xa);
-        fp4_word_to_h2(wb[2 * q + w], xb);
+      for (int j = 0; j < 4; ++j) {
+        xa[j] = h2_mul(xa[j], sca[w >> 1]);
+        xb[j] = h2_mul(xb[j], scb[w >> 1]);
+      }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          xa[j] = h2_mul(xa[j], sa);
-          xb[j] = h2_mul(xb[j], sb);
-        }
-        const int k = 4 * q + 2 * w;
-#pragma unroll
-        for (int p = 0; p < SPLIT; ++p) {
-          mma_16816_f16(s0, xa[0], xb[0], xa[1], xb[1], qf[p][k][0], qf[p][k][1]);
-          mma_16816_f16(s1, xa[2], xb[2], xa[3], xb[3], qf[p][k + 1][0], qf[p][k + 1][1]);
-        }
+      for (int p = 0; p < SPLIT; ++p) {
+        mma_16816_f16(s0, xa[0], xb[0], xa[1], xb[1], qf[p][2 * w][0], qf[p][2 * w][1]);
+        mma_16816_f16(s1, xa[2], xb[2], xa[3], xb[3], qf[p][2 * w + 1][0], qf[p][2 * w + 1][1]);
       }
     }
-  }
-  // x[0]: (token g, column 2t) x[1]: (g, 2t+1) x[2]: (g+8, 2t) x[3]: (g+8, 2t+1)
-  float x[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = (s0[i] + s1[i]) * qs[i & 1];
-  if (nt < kFp4Tok) {
-    if (g >= nt) x[0] = x[1] = kNegInf;
-    if (g + 8 >= nt) x[2] = x[3] = kNegInf;
+    for (int i = 0; i < 4; ++i) x[u][i] = (s0[i] + s1[i]) * qs[i & 1];
+    if constexpr (PART) {
+      if (16 * u + g >= nt) x[u][0] = x[u][1] = kNegInf;
+      if (16 * u + g + 8 >= nt) x[u][2] = x[u][3] = kNegInf;
+    }
   }
-  const float cm[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+  float cm[2] = {fmaxf(x[0][0], x[0][2]), fmaxf(x[0][1], x[0][3])};
+#pragma unroll
+  for (int u = 1; u < NU; ++u) {
+    cm[0] = fmaxf(cm[0], fmaxf(x[u][0], x[u][2]));
+    cm[1] = fmaxf(cm[1], fmaxf(x[u][1], x[u][3]));
+  }
   const bool grow = cm[0] > mref[0] + 15.f || cm[1] > mref[1] + 15.f;
   if (__any_sync(FULL, grow)) {
 #pragma unroll
@@ -165,7 +187,7 @@ __device__ __forceinline__ void fp4_unit(const uint8_t* row0, uint32_t pitch, ui
       v = fmaxf(v, __shfl_xor_sync(FULL, v, 8));
       v = fmaxf(v, __shfl_xor_sync(FULL, v, 16));
       if (v > mref[n] + 15.f) {  // the same decision on every lane of the column
-        const float alpha = (mref[n] == kNegInf) ? 0.f : exp2f(mref[n] - (v - 7.f));
+        const float alpha = (mref[n] == kNegInf) ? 0.f : ex2_approx(mref[n] - (v - 7.f));
         mref[n] = v - 7.f;
         lsum[n] *= alpha;
 #pragma unroll
@@ -176,47 +198,56 @@ __device__ __forceinline__ void fp4_unit(const uint8_t* row0, uint32_t pitch, ui
       }
     }
   }
-  float p[4];
+  uint32_t pb[NU][SPLIT][2];  // P^T as the B operand: tokens 0-7 and 8-15 of each unit
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = (x[i] == kNegInf) ? 0.f : exp2f(x[i] - mref[i & 1]);
-  lsum[0] += p[0] + p[2];
-  lsum[1] += p[1] + p[3];
-  uint32_t pb[SPLIT][2];
-  {
+  for (int u = 0; u < NU; ++u) {
+    float p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[i] = ex2_approx(x[u][i] - mref[i & 1]);
+      if (PART) p[i] = (x[u][i] == kNegInf) ? 0.f : p[i];  // a column without a token yet: -inf - -inf
+    }
+    lsum[0] += p[0] + p[2];
+    lsum[1] += p[1] + p[3];
     const uint32_t h0 = pack_h2(p[0], p[1]), h1 = pack_h2(p[2], p[3]);
-    pb[0][0] = movmatrix_trans(h0);  // tokens 0-7
-    pb[0][1] = movmatrix_trans(h1);  // tokens 8-15
+    pb[u][0][0] = movmatrix_trans(h0);
+    pb[u][0][1] = movmatrix_trans(h1);
     if constexpr (SPLIT == 2) {
       const float2 f0 = h2_to_f2(h0), f1 = h2_to_f2(h1);
-      pb[1][0] = movmatrix_trans(pack_h2(p[0] - f0.x, p[1] - f0.y));
-      pb[1][1] = movmatrix_trans(pack_h2(p[2] - f1.x, p[3] - f1.y));
+      pb[u][1][0] = movmatrix_trans(pack_h2(p[0] - f0.x, p[1] - f0.y));
+      pb[u][1][1] = movmatrix_trans(pack_h2(p[2] - f1.x, p[3] - f1.y));
     }
   }
-  // ---- O^T: features [g D/8, (g+1) D/8) of tokens 2t, 2t+1, 2t+8, 2t+9
-  {
-    constexpr int NW = D / 64;  // words of codes per token
-    uint32_t lo[2][NW], hi[2][NW], sc[2][D > 128 ? 2 : 1];
+  // ---- O^T: features [g D/8, (g+1) D/8) of tokens 2t, 2t+1, 2t+8, 2t+9 of each unit
+  constexpr int NW = D / 64;               // words of codes per token
+  constexpr int NS = D > 128 ? 2 : 1;      // scales per token
+  const uint8_t* vrow = row0 + (uint32_t)(2 * t) * pitch + code_off + D / 2 + g * (D / 16);
+  const uint8_t* wrow = row0 + (uint32_t)(2 * t) * pitch + scale_off + D / 16 + (g * (D / 8)) / 16;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int ta = 2 * t + 8 * u;
-      const uint8_t* ra = row0 + (uint32_t)ta * pitch;
-      const uint8_t* rb = ra + pitch;
+  for (int u = 0; u < NU; ++u) {
+    uint32_t lo[2][NW], hi[2][NW], sc[2][NS];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int ta = 16 * u + 8 * b;  // token pair (ta + 2t, ta + 2t + 1)
       uint32_t wa[NW], wb[NW];
-      fp4_lds<NW>(ra + code_off + D / 2 + g * (D / 16), wa);
-      fp4_lds<NW>(rb + code_off + D / 2 + g * (D / 16), wb);
+      fp4_lds<NW>(vrow + (uint32_t)ta * pitch, wa);
+      fp4_lds<NW>(vrow + (uint32_t)(ta + 1) * pitch, wb);
 #pragma unroll
-      for (int q = 0; q < (D > 128 ? 2 : 1); ++q) {
-        const uint32_t so = scale_off + D / 16 + (g * (D / 8)) / 16 + q;
-        // rows past the last token hold whatever the stage held before: a zero scale
-        // keeps their products finite (their weights are zero)
-        const uint32_t sa8 = ta < nt ? ra[so] : 0u, sb8 = ta + 1 < nt ? rb[so] : 0u;
-        sc[u][q] = fp4_scale2_to_h2(sa8 | (sb8 << 8));
+      for (int q = 0; q < NS; ++q) {
+        uint32_t sa = wrow[(uint32_t)ta * pitch + q], sb = wrow[(uint32_t)(ta + 1) * pitch + q];
+        if constexpr (PART) {
+          // rows past the last token hold whatever the stage held before: a zero scale
+          // keeps their products finite (their weights are zero)
+          if (ta + 2 * t >= nt) sa = 0;
+          if (ta + 2 * t + 1 >= nt) sb = 0;
+        }
+        sc[b][q] = fp4_scale2_to_h2(sa | (sb << 8));
       }
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         // bytes of (token a, token b) codes: even features, odd features
-        lo[u][w] = (wa[w] & 0x0f0f0f0fu) | ((wb[w] & 0x0f0f0f0fu) << 4);
-        hi[u][w] = ((wa[w] >> 4) & 0x0f0f0f0fu) | (wb[w] & 0xf0f0f0f0u);
+        lo[b][w] = (wa[w] & 0x0f0f0f0fu) | ((wb[w] << 4) & 0xf0f0f0f0u);
+        hi[b][w] = ((wa[w] >> 4) & 0x0f0f0f0fu) | (wb[w] & 0xf0f0f0f0u);
       }
     }
 #pragma unroll
@@ -232,18 +263,19 @@ __device__ __forceinline__ void fp4_unit(const uint8_t* row0, uint32_t pitch, ui
         const uint32_t a0 = h2_mul(l0[j], sc[0][q]), a1 = h2_mul(h0[j], sc[0][q]);
         const uint32_t a2 = h2_mul(l1[j], sc[1][q]), a3 = h2_mul(h1[j], sc[1][q]);
 #pragma unroll
-        for (int pp = 0; pp < SPLIT; ++pp) mma_16816_f16(acc[4 * w + j], a0, a1, a2, a3, pb[pp][0], pb[pp][1]);
+        for (int pp = 0; pp < SPLIT; ++pp) mma_16816_f16(acc[4 * w + j], a0, a1, a2, a3, pb[u][pp][0], pb[u][pp][1]);
       }
     }
   }
 }
 
 template <typename T, int D, int NCW>
-__global__ void __launch_bounds__((NCW + 1) * 32, 1) decode_fp4_kernel(const DecodeArgs a, const float v_scale) {
+__global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const DecodeArgs a, const float v_scale) {
   // programmatic dependent launch exactly as decode_kernel: the plan and the page ids are
   // read before the wait, everything the previous kernel may have written after it
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int SPLIT = sizeof(T) == 4 ? 2 : 1;
+  constexpr int NU = fp4_units_of(NCW), TW = 16 * NU;
   constexpr int KS = D / 16;
   constexpr unsigned FULL = 0xffffffffu;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -272,7 +304,13 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 1) decode_fp4_kernel(const Dec
   const int P = 1 << a.page_log2;
   const int TS = a.TS;
 
-  if (warp == NCW) {
+  // Register split: NCW + 4 warps launch with 96 (NCW 16) or 168 (NCW 8) registers a thread;
+  // the consumers take 112 (232) and the last warpgroup, of which one warp works, keeps 32
+  // (40): 512 x 112 + 128 x 32 = 640 x 96, and 256 x 232 + 128 x 40 = 384 x 168.
+  if (warp >= NCW) {
+    if constexpr (NCW == 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp > NCW) return;
     // ------------------------------------------------------------ producer
     const uint64_t pol = l2_evict_first_policy();
     const uint8_t* pool = reinterpret_cast<const uint8_t*>(a.k_pool);
@@ -354,13 +392,16 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 1) decode_fp4_kernel(const Dec
   }
 
   // -------------------------------------------------------------- consumers
+  if constexpr (NCW == 16) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
   const int h = warp / a.WPH;
   const int sub = warp - h * a.WPH;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t code_off = fp4_code_off(h, D), scale_off = fp4_scale_off(h, a.Hkv, D);
   float* cbuf = reinterpret_cast<float*>(smem + L.cbuf);
   const T* qbase = reinterpret_cast<const T*>(a.q);
-  int ctr = 0;
+  int st = 0;
+  uint32_t ph = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // q, the workspace and out follow the previous kernel
   for (int i = 0; i < seg1 - seg0; ++i) {
     const int si = decode_seg_at(a, seg0, seg1, last_first, i);
@@ -410,20 +451,28 @@ __global__ void __launch_bounds__((NCW + 1) * 32, 1) decode_fp4_kernel(const Dec
     float mref[2] = {kNegInf, kNegInf}, lsum[2] = {0.f, 0.f};
     for (int tok = 0; tok < ntok; tok += TS) {
       const int nt = min(TS, ntok - tok);
-      const int st = ctr % a.NSTAGE;
-      const uint32_t ph = (uint32_t)(ctr / a.NSTAGE) & 1u;
-      bool ok = __all_sync(FULL, *s_abort == 0);
-      if (ok) ok = __all_sync(FULL, mbar_wait(&full[st], ph, kWdDecodeFull));
-      if (!ok) *s_abort = 1;
+      bool ok = mbar_try_wait(&full[st], ph);
+      if (!__all_sync(FULL, ok)) {
+        ok = __all_sync(FULL, *s_abort == 0);
+        if (ok) ok = __all_sync(FULL, mbar_wait(&full[st], ph, kWdDecodeFull));
+        if (!ok) *s_abort = 1;
+      }
       if (ok) {
         const uint8_t* rows = smem + (size_t)st * a.stage_bytes;
-        for (int t0 = sub * kFp4Tok; t0 < nt; t0 += a.WPH * kFp4Tok)
-          fp4_unit<D, SPLIT>(rows + (size_t)t0 * a.row_bytes, a.row_bytes, code_off, scale_off,
-                             min(kFp4Tok, nt - t0), lane, qs, qf, acc, mref, lsum);
+        for (int t0 = sub * TW; t0 < nt; t0 += a.WPH * TW) {
+          const uint8_t* row0 = rows + (uint32_t)t0 * a.row_bytes;
+          if (nt - t0 >= TW)
+            fp4_units<D, SPLIT, NU, false>(row0, a.row_bytes, code_off, scale_off, TW, lane, qs, qf, acc, mref, lsum);
+          else
+            fp4_units<D, SPLIT, NU, true>(row0, a.row_bytes, code_off, scale_off, nt - t0, lane, qs, qf, acc, mref, lsum);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
-      ++ctr;
+      if (++st == a.NSTAGE) {
+        st = 0;
+        ph ^= 1u;
+      }
     }
     // ---- row sums over the 8 lanes of each head column
 #pragma unroll
