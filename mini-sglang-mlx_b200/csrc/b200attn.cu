@@ -1100,7 +1100,7 @@ int fp4_decode_config(int Hq, int Hkv, int D, DecodeCfg& c) {
   c.NCW = Hkv == 16 ? 16 : 8;
   c.WPH = c.NCW / Hkv;
   // a stage holds what every warp takes at a time, more while it stays near 40 KB
-  c.TS = 16 * b2a::fp4_units_of(c.NCW) * c.WPH;
+  c.TS = 16 * b2a::fp4_units_of(c.NCW, D) * c.WPH;
   while (2u * c.TS * c.row_bytes <= 40960u) c.TS *= 2;
   c.stage_bytes = (uint32_t)c.TS * c.row_bytes;
   const size_t fixed = b2a::fp4_decode_smem(0, c.stage_bytes, c.NCW, c.WPH, G, D).total + 6 * 16;

@@ -9,7 +9,7 @@
 // What bounds it. A cached value is 0.56 bytes, so at HBM rate an SM receives
 // about 40 values per clock (1.13 bytes and 2 G multiply-adds per K/V pair):
 // expanding and multiplying them has to cost less than a clock per 40 values.
-// One warp takes one or two units of 16 tokens x one kv head at a time; a unit is
+// One warp takes one to four units of 16 tokens x one kv head at a time; a unit is
 //   S^T [16 tokens x 8 head columns] = K [16 x D] . Q^T      (D/16 MMAs)
 //   O^T [D x 8]                     += V^T [D x 16] . P^T    (D/16 MMAs)
 // with mma.sync m16n8k16, fp16 in, fp32 accumulate. The codes become MMA
@@ -38,7 +38,10 @@
 namespace b2a {
 
 // units of 16 tokens a warp takes at a time
-__host__ __device__ constexpr int fp4_units_of(int NCW) { return NCW == 16 ? 1 : 2; }
+// (measured at 8 kv heads x 128, 72 requests of 16k tokens: 332, 330, 282 us for 1, 2, 4
+// units; 16 warps of 2 units, which need a combine per segment: 303 us). Four units of
+// head_dim 256 would leave room for one stage, and 16 warps have registers for one unit.
+__host__ __device__ constexpr int fp4_units_of(int NCW, int D) { return NCW == 16 ? 1 : D == 256 ? 2 : 4; }
 
 struct Fp4DecodeSmem {
   uint32_t bars, cbuf, abort_flag, last_flag, total;
@@ -56,7 +59,7 @@ __host__ __device__ inline Fp4DecodeSmem fp4_decode_smem(int NSTAGE, uint32_t st
   off = (off + 15u) & ~15u;
   L.abort_flag = off;
   L.last_flag = off + 16;
-  L.total = off + 32;
+  L.total = off + 32;  // last_flag: one word per pending request
   return L;
 }
 
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const Dec
   // read before the wait, everything the previous kernel may have written after it
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int SPLIT = sizeof(T) == 4 ? 2 : 1;
-  constexpr int NU = fp4_units_of(NCW), TW = 16 * NU;
+  constexpr int NU = fp4_units_of(NCW, D), TW = 16 * NU;
   constexpr int KS = D / 16;
   constexpr unsigned FULL = 0xffffffffu;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -331,12 +334,6 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const Dec
         const int nt = min(TS, ntok - tok);
         const int st = ctr % a.NSTAGE;
         const uint32_t ph = (uint32_t)(ctr / a.NSTAGE) & 1u;
-        if (!__all_sync(FULL, mbar_wait(&empty[st], ph ^ 1u, kWdDecodeEmpty))) {
-          *s_abort = 1;
-          ok = false;
-          break;
-        }
-        uint8_t* dst = smem + (size_t)st * a.stage_bytes;
         // a run inside one page (P >= TS), or whole pages (stages start on page boundaries)
         const bool one_run = P >= TS;
         const int ncopies = one_run ? 1 : ((nt + P - 1) >> a.page_log2);
@@ -351,6 +348,13 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const Dec
           good = good && page >= 0 && s0 + rows <= a.num_slots;
         }
         good = __all_sync(FULL, good);
+        // the page ids are read (and checked) while the stage is still in use
+        if (!__all_sync(FULL, mbar_wait(&empty[st], ph ^ 1u, kWdDecodeEmpty))) {
+          *s_abort = 1;
+          ok = false;
+          break;
+        }
+        uint8_t* dst = smem + (size_t)st * a.stage_bytes;
         if (lane == 0) {
           if (good) {
             mbar_arrive_expect_tx(&full[st], (uint32_t)nt * a.row_bytes);
@@ -403,14 +407,15 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const Dec
   int st = 0;
   uint32_t ph = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // q, the workspace and out follow the previous kernel
+  const int4* segs = reinterpret_cast<const int4*>(a.segs);
+  int4 next = seg1 > seg0 ? segs[decode_seg_at(a, seg0, seg1, last_first, 0)] : make_int4(0, 0, 0, -1);
+  int pend[2] = {0, 0}, npend = 0;  // requests whose partial rows this CTA has written, tickets not yet taken
   for (int i = 0; i < seg1 - seg0; ++i) {
-    const int si = decode_seg_at(a, seg0, seg1, last_first, i);
-    int b, pbeg, ntok, slot;
-    decode_get_seg(a, si, b, pbeg, ntok, slot);
-    if (!decode_seg_ok(a, b, slot)) {
-      if (threadIdx.x == 0) watchdog_set(kWdBadPlan);
-      continue;
-    }
+    const int b = next.x, ntok = next.z, slot = next.w;
+    if (i + 1 < seg1 - seg0) next = segs[decode_seg_at(a, seg0, seg1, last_first, i + 1)];
+    const bool good = decode_seg_ok(a, b, slot);
+    if (!good && threadIdx.x == 0) watchdog_set(kWdBadPlan);
+    if (good) {
     // ---- Q^T: head column g, features [t D/4, (t+1) D/4); zero columns past the group
     uint32_t qf[SPLIT][KS][2];
     float qs[2];
@@ -445,6 +450,14 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const Dec
       qs[0] = __shfl_sync(FULL, inv, 8 * t);      // column 2t
       qs[1] = __shfl_sync(FULL, inv, 8 * t + 4);  // column 2t + 1
     }
+    // the next segment's query row and merge range come closer while this one is streamed
+    if (i + 1 < seg1 - seg0 && next.x >= 0 && next.x < a.B) {
+      if (g < G) {
+        const T* qn = qbase + ((size_t)next.x * a.Hq + h * G + g) * D + t * (D / 4);
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(qn));
+        if (next.w >= 0) asm volatile("prefetch.global.L1 [%0];" ::"l"(a.merge_indptr + next.x));
+      }
+    }
     float acc[KS][4];
 #pragma unroll
     for (int mt = 0; mt < KS; ++mt) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
@@ -461,10 +474,17 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const Dec
         const uint8_t* rows = smem + (size_t)st * a.stage_bytes;
         for (int t0 = sub * TW; t0 < nt; t0 += a.WPH * TW) {
           const uint8_t* row0 = rows + (uint32_t)t0 * a.row_bytes;
-          if (nt - t0 >= TW)
+          if (nt - t0 >= TW) {
             fp4_units<D, SPLIT, NU, false>(row0, a.row_bytes, code_off, scale_off, TW, lane, qs, qf, acc, mref, lsum);
-          else
-            fp4_units<D, SPLIT, NU, true>(row0, a.row_bytes, code_off, scale_off, nt - t0, lane, qs, qf, acc, mref, lsum);
+          } else {
+            // the rows that are left, unit by unit: little code beside the full step (a second
+            // copy of it costs instruction-cache misses)
+#pragma unroll 1
+            for (int t1 = t0; t1 < nt; t1 += 16) {
+              fp4_units<D, SPLIT, 1, true>(row0, a.row_bytes, code_off, scale_off, nt - t1, lane, qs, qf, acc, mref, lsum);
+              row0 += 16u * a.row_bytes;
+            }
+          }
         }
       }
       __syncwarp();
@@ -547,23 +567,32 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const Dec
       }
       if (slot >= 0) __threadfence();  // publish the partial rows at GPU scope before the ticket
     }
-    if (slot >= 0) {
-      // merge ticket of request b, as in decode_kernel
-      named_bar_sync(1, NCW * 32);
-      const int p0 = a.merge_indptr[b], p1 = a.merge_indptr[b + 1];
-      if (threadIdx.x == 0) {
+    if (a.WPH > 1) named_bar_sync(1, NCW * 32);  // cbuf is free again
+    if (slot >= 0) pend[npend++] = b;
+    }
+    // Tickets of the pending requests, and the merge of those that this CTA completes: at the end
+    // of the CTA's work (a share cuts at most two requests), because they cost all warps a fence,
+    // two barriers and an atomic round trip.
+    if (npend == 2 || (npend > 0 && i + 1 == seg1 - seg0)) {
+      named_bar_sync(1, NCW * 32);  // every warp has written and fenced its rows
+      if (threadIdx.x < (unsigned)npend) {
+        const int pb = threadIdx.x ? pend[1] : pend[0];
+        const int p0 = a.merge_indptr[pb], p1 = a.merge_indptr[pb + 1];
         const int prev = atomicAdd(&a.tickets[p0], 1);
         const bool last = prev == p1 - p0 - 1;
         if (last) a.tickets[p0] = 0;  // every partial has arrived: re-arm for the next call
-        *s_last = last ? 1 : 0;
+        s_last[threadIdx.x] = last ? 1 : 0;
       }
       named_bar_sync(1, NCW * 32);
-      if (*s_last) {
-        __threadfence();
-        decode_merge_request<T, D>(a, b, p0, p1, warp, lane);
+#pragma unroll 1
+      for (int k = 0; k < npend; ++k) {
+        const int pb = k ? pend[1] : pend[0];
+        if (s_last[k]) {
+          __threadfence();
+          decode_merge_request<T, D>(a, pb, a.merge_indptr[pb], a.merge_indptr[pb + 1], warp, lane);
+        }
       }
-    } else if (a.WPH > 1) {
-      named_bar_sync(1, NCW * 32);
+      npend = 0;
     }
   }
 }
