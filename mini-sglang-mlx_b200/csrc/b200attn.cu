@@ -1462,9 +1462,9 @@ int b2a_extend_metadata(const int32_t* page_table, int64_t table_rows, int64_t t
   const size_t smem = b2a::extend_meta_smem(B);
   if (int rc = ensure_smem((const void*)b2a::extend_meta_kernel, b2a::extend_meta_smem(b2a::kEmMaxBatch), "extend_meta"))
     return rc;
-  // enough threads for one walk each over tokens and pages, at most two CTAs per SM
-  const int64_t walks = (std::max(q_capacity, idx_capacity) + b2a::kEmVec - 1) / b2a::kEmVec;
-  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(2 * 148, (walks + b2a::kEmThreads - 1) / b2a::kEmThreads));
+  // a thread per token, page or sixteenth of a tile, at most two CTAs per SM
+  const int64_t elems = std::max({q_capacity, idx_capacity, (int64_t)16 * work_capacity});
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(2 * 148, (elems + b2a::kEmThreads - 1) / b2a::kEmThreads));
   b2a::extend_meta_kernel<<<(unsigned)grid, b2a::kEmThreads, smem, reinterpret_cast<cudaStream_t>(stream)>>>(a);
   return check_launch("extend_meta_kernel");
 }

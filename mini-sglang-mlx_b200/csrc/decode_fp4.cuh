@@ -139,13 +139,14 @@ __device__ __forceinline__ void fp4_units(const uint8_t* row0, uint32_t pitch, u
   constexpr int KS = D / 16;  // MMAs of a product
   const int g = lane >> 2, t = lane & 3;
   // ---- S^T: rows g and g + 8 of each unit, features [t D/4, (t+1) D/4)
-  // x[u][0]: (token g, column 2t) [1]: (g, 2t+1) [2]: (g+8, 2t) [3]: (g+8, 2t+1)
+  // raw scores, x[u][0]: (token g, column 2t) [1]: (g, 2t+1) [2]: (g+8, 2t) [3]: (g+8, 2t+1)
   float x[NU][4];
   const uint8_t* krow = row0 + (uint32_t)g * pitch + code_off + t * (D / 8);
   const uint8_t* srow = row0 + (uint32_t)g * pitch + scale_off + t * (D / 64);
 #pragma unroll
   for (int u = 0; u < NU; ++u) {
-    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[u][i] = 0.f;
     uint32_t wa[D / 32], wb[D / 32];
     fp4_lds<D / 32>(krow + (16u * u) * pitch, wa);
     fp4_lds<D / 32>(krow + (16u * u + 8u) * pitch, wb);
@@ -164,12 +165,10 @@ __device__ __forceinline__ void fp4_units(const uint8_t* row0, uint32_t pitch, u
       }
 #pragma unroll
       for (int p = 0; p < SPLIT; ++p) {
-        mma_16816_f16(s0, xa[0], xb[0], xa[1], xb[1], qf[p][2 * w][0], qf[p][2 * w][1]);
-        mma_16816_f16(s1, xa[2], xb[2], xa[3], xb[3], qf[p][2 * w + 1][0], qf[p][2 * w + 1][1]);
+        mma_16816_f16(x[u], xa[0], xb[0], xa[1], xb[1], qf[p][2 * w][0], qf[p][2 * w][1]);
+        mma_16816_f16(x[u], xa[2], xb[2], xa[3], xb[3], qf[p][2 * w + 1][0], qf[p][2 * w + 1][1]);
       }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[u][i] = (s0[i] + s1[i]) * qs[i & 1];
     if constexpr (PART) {
       if (16 * u + g >= nt) x[u][0] = x[u][1] = kNegInf;
       if (16 * u + g + 8 >= nt) x[u][2] = x[u][3] = kNegInf;
@@ -181,6 +180,8 @@ __device__ __forceinline__ void fp4_units(const uint8_t* row0, uint32_t pitch, u
     cm[0] = fmaxf(cm[0], fmaxf(x[u][0], x[u][2]));
     cm[1] = fmaxf(cm[1], fmaxf(x[u][1], x[u][3]));
   }
+  cm[0] *= qs[0];  // qs > 0 keeps the order
+  cm[1] *= qs[1];
   const bool grow = cm[0] > mref[0] + 15.f || cm[1] > mref[1] + 15.f;
   if (__any_sync(FULL, grow)) {
 #pragma unroll
@@ -207,7 +208,7 @@ __device__ __forceinline__ void fp4_units(const uint8_t* row0, uint32_t pitch, u
     float p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      p[i] = ex2_approx(x[u][i] - mref[i & 1]);
+      p[i] = ex2_approx(fmaf(x[u][i], qs[i & 1], -mref[i & 1]));
       if (PART) p[i] = (x[u][i] == kNegInf) ? 0.f : p[i];  // a column without a token yet: -inf - -inf
     }
     lsum[0] += p[0] + p[2];
@@ -318,75 +319,88 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const Dec
     const uint64_t pol = l2_evict_first_policy();
     const uint8_t* pool = reinterpret_cast<const uint8_t*>(a.k_pool);
     const size_t rowB = a.row_bytes;
-    int ctr = 0;
-    bool ok = true;
+    // a stage is a run inside one page (P >= TS), or whole pages (stages start on page boundaries)
+    const bool one_run = P >= TS;
+    const int nseg = seg1 - seg0;
+    int seg = -1, tok = 0, ntok = 0, pbeg = 0;
+    auto advance = [&]() -> bool {  // to the next stage
+      tok += TS;
+      while (tok >= ntok) {
+        if (++seg >= nseg) return false;
+        int b, slot;
+        decode_get_seg(a, decode_seg_at(a, seg0, seg1, last_first, seg), b, pbeg, ntok, slot);
+        if (!decode_seg_ok(a, b, slot)) ntok = 0;  // the consumers skip it too (and report it)
+        tok = 0;
+      }
+      return true;
+    };
+    auto copies = [&](int nt) { return one_run ? 1 : (nt + P - 1) >> a.page_log2; };
+    auto first_id = [&]() -> int {  // this lane's page id of the stage at (seg, tok)
+      return lane < copies(min(TS, ntok - tok)) ? a.kv_indices[pbeg + (tok >> a.page_log2) + lane] : -2;
+    };
+    int ctr = 0, st = 0;
+    uint32_t ph = 1;
     bool waited = false;
-    for (int i = 0; i < seg1 - seg0 && ok; ++i) {
-      const int si = decode_seg_at(a, seg0, seg1, last_first, i);
-      int b, pbeg, ntok, slot;
-      decode_get_seg(a, si, b, pbeg, ntok, slot);
-      if (!decode_seg_ok(a, b, slot)) continue;  // the consumers skip it too (and report it)
-      for (int tok = 0; tok < ntok; tok += TS) {
-        if (!__all_sync(FULL, *s_abort == 0)) {
-          ok = false;
-          break;
-        }
-        const int nt = min(TS, ntok - tok);
-        const int st = ctr % a.NSTAGE;
-        const uint32_t ph = (uint32_t)(ctr / a.NSTAGE) & 1u;
-        // a run inside one page (P >= TS), or whole pages (stages start on page boundaries)
-        const bool one_run = P >= TS;
-        const int ncopies = one_run ? 1 : ((nt + P - 1) >> a.page_log2);
-        const int first_page = pbeg + (tok >> a.page_log2);
-        // bad page ids never reach the copy engine: the error is recorded, the stage's
-        // copies are skipped and the consumers run on what the stage held
-        bool good = true;
-        for (int j = lane; j < ncopies; j += 32) {
-          const int64_t page = a.kv_indices[first_page + j];
-          const int64_t s0 = one_run ? page * P + (tok & (P - 1)) : page * P;
-          const int rows = one_run ? nt : min(P, nt - j * P);
-          good = good && page >= 0 && s0 + rows <= a.num_slots;
-        }
-        good = __all_sync(FULL, good);
-        // the page ids are read (and checked) while the stage is still in use
-        if (!__all_sync(FULL, mbar_wait(&empty[st], ph ^ 1u, kWdDecodeEmpty))) {
-          *s_abort = 1;
-          ok = false;
-          break;
-        }
-        uint8_t* dst = smem + (size_t)st * a.stage_bytes;
-        if (lane == 0) {
-          if (good) {
-            mbar_arrive_expect_tx(&full[st], (uint32_t)nt * a.row_bytes);
-          } else {
-            watchdog_set(kWdBadSlot);
-            mbar_arrive(&full[st]);
-          }
-        }
-        __syncwarp();
-        if (!waited) {
-          asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows of the previous kernel
-          waited = true;
-        }
+    bool have = advance();
+    int id = have ? first_id() : -2;
+    while (have) {
+      const int nt = min(TS, ntok - tok);
+      const int ncopies = copies(nt);
+      const int32_t* ids = a.kv_indices + pbeg + (tok >> a.page_log2);
+      const int in_page = one_run ? tok & (P - 1) : 0;
+      const int my_id = id;
+      // the next stage's segment and page ids are on their way while this stage waits and copies
+      have = advance();
+      id = have ? first_id() : -2;
+      // bad page ids never reach the copy engine: the error is recorded, the stage's
+      // copies are skipped and the consumers run on what the stage held
+      bool good = true;
+      for (int j = lane; j < ncopies; j += 32) {
+        const int64_t page = j < 32 ? my_id : ids[j];
+        const int rows = one_run ? nt : min(P, nt - j * P);
+        good = good && page >= 0 && page * P + in_page + rows <= a.num_slots;
+      }
+      good = __all_sync(FULL, good);
+      if (!__all_sync(FULL, mbar_wait(&empty[st], ph, kWdDecodeEmpty)) || !__all_sync(FULL, *s_abort == 0)) {
+        *s_abort = 1;
+        break;
+      }
+      uint8_t* dst = smem + (size_t)st * a.stage_bytes;
+      if (lane == 0) {
         if (good) {
-          for (int j0 = 0; j0 < ncopies; j0 += 32) {
-            // consecutive page ids are consecutive slots: one bulk copy per run of them
-            const int j = j0 + lane;
-            const int64_t page = j < ncopies ? a.kv_indices[first_page + j] : -2;
-            const int64_t prev = __shfl_up_sync(FULL, page, 1);
-            const bool head = j < ncopies && (lane == 0 || page != prev + 1);
-            const uint32_t heads = __ballot_sync(FULL, head);
-            if (head) {
-              const uint32_t above = lane == 31 ? 0u : (heads >> (lane + 1)) << (lane + 1);
-              const int end = j0 + (above ? __ffs((int)above) - 1 : min(32, ncopies - j0));
-              const int rows = one_run ? nt : min(end * P, nt) - j * P;
-              const int64_t s0 = one_run ? page * P + (tok & (P - 1)) : page * P;
-              bulk_g2s(dst + (size_t)j * P * rowB, pool + s0 * rowB, (uint32_t)rows * a.row_bytes, &full[st], pol);
-            }
+          mbar_arrive_expect_tx(&full[st], (uint32_t)nt * a.row_bytes);
+        } else {
+          watchdog_set(kWdBadSlot);
+          mbar_arrive(&full[st]);
+        }
+      }
+      __syncwarp();
+      if (!waited) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows of the previous kernel
+        waited = true;
+      }
+      if (good) {
+        for (int j0 = 0; j0 < ncopies; j0 += 32) {
+          // consecutive page ids are consecutive slots: one bulk copy per run of them
+          const int j = j0 + lane;
+          const int64_t page = j < ncopies ? (j0 == 0 ? my_id : ids[j]) : -2;
+          const int64_t prev = __shfl_up_sync(FULL, page, 1);
+          const bool head = j < ncopies && (lane == 0 || page != prev + 1);
+          const uint32_t heads = __ballot_sync(FULL, head);
+          if (head) {
+            const uint32_t above = lane == 31 ? 0u : (heads >> (lane + 1)) << (lane + 1);
+            const int end = j0 + (above ? __ffs((int)above) - 1 : min(32, ncopies - j0));
+            const int rows = one_run ? nt : min(end * P, nt) - j * P;
+            bulk_g2s(dst + (size_t)j * P * rowB, pool + (page * P + in_page) * rowB, (uint32_t)rows * a.row_bytes,
+                     &full[st], pol);
           }
         }
-        __syncwarp();
-        ++ctr;
+      }
+      __syncwarp();
+      ++ctr;
+      if (++st == a.NSTAGE) {
+        st = 0;
+        ph ^= 1u;
       }
     }
     // never leave while our own copies may still be landing

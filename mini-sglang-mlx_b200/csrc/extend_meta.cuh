@@ -13,13 +13,14 @@
 //                          in request order
 //
 // One launch. It moves a few bytes per token and page, so what bounds a usual batch is
-// latency: launches, and the chain scan -> search -> table entry. Every CTA therefore
-// scans all B requests itself (12 bytes each, from L2) into shared memory instead of
-// waiting for another CTA or launch to do it, finds the requests of its slice of tokens,
-// pages and tiles by binary search there, and walks on from the first. A tile's place in
-// the sorted list is the number of tiles that go before it, counted directly: all keys
-// are unique (cost, then order), so no two tiles claim one place and no order of
-// execution matters.
+// latency: the launch, and the chain lengths -> scan -> search -> table entry. Every CTA
+// therefore scans all B requests itself (12 bytes each, from L2) into shared memory
+// instead of waiting for another CTA or launch to do it, and finds the owners of its
+// tokens, pages and tiles by binary search there, four at a time so that their searches
+// and table reads overlap. A tile's place in the sorted list is the number of tiles that
+// go before it, counted directly: all keys are unique (cost, then order), so no two tiles
+// claim one place and no order of execution matters. A warp counts for up to eight tiles at
+// once, reading every key from shared memory once.
 #pragma once
 
 #include "common.cuh"
@@ -27,11 +28,11 @@
 namespace b2a {
 
 constexpr int kEmThreads = 256;
-constexpr int kEmMaxBatch = 8192;  // three int32 prefix arrays of a batch in shared memory
+constexpr int kEmMaxBatch = 8192;  // five int32 arrays of a batch in shared memory
 constexpr int kEmKeys = 2048;      // tile keys compared per round
+constexpr int kEmOwn = 8;          // tiles a warp ranks at once
 constexpr int kEmMaxTile = 256;    // cost < 2^39, so (cost, order) fits 64 bits
 constexpr int kEmMaxWork = 1 << 24;
-constexpr int kEmVec = 4;          // tokens, pages or tiles a thread walks from one search
 
 struct ExtendMetaArgs {
   const int32_t* page_table;
@@ -55,23 +56,7 @@ struct ExtendMetaArgs {
 };
 
 __host__ __device__ inline size_t extend_meta_smem(int B) {
-  return (size_t)kEmKeys * 8 + 3 * (size_t)(B + 1) * 4;
-}
-
-struct EmReq {
-  int cached, ext, pages;
-};
-
-// Lengths of request b, forced into the table's range (flagged once, by CTA 0).
-__device__ __forceinline__ EmReq em_request(const ExtendMetaArgs& a, int b) {
-  int L = a.lens[b], c = a.cached[b];
-  const bool bad = L < 0 || (int64_t)L > a.stride || c < 0 || c > L || a.rows[b] < 0 || a.rows[b] >= a.table_rows;
-  if (bad) {
-    if (blockIdx.x == 0) watchdog_set(kWdMetaOverflow);
-    L = L < 0 ? 0 : (int)min((int64_t)L, a.stride);
-    c = min(max(c, 0), L);
-  }
-  return {c, L - c, (int)(((int64_t)L + (1 << a.page_log2) - 1) >> a.page_log2)};
+  return (size_t)kEmKeys * 8 + 5 * (size_t)(B + 1) * 4;
 }
 
 // Last b in [0, B) with pre[b] <= x (pre ascending, pre[0] = 0): the owner of element x
@@ -86,43 +71,59 @@ __device__ __forceinline__ int em_find(const int32_t* pre, int B, int x) {
   return lo;
 }
 
-// Key of tile i of request b: dearer tiles and, among equals, earlier tiles are larger.
-__device__ __forceinline__ unsigned long long em_key(const ExtendMetaArgs& a, const int32_t* qo, int b, int k, int i,
-                                                     int& tb, int& nq) {
-  const int ext = qo[b + 1] - qo[b];
-  tb = k * a.tile_q;
-  nq = min(a.tile_q, ext - tb);
-  const unsigned long long cost = (unsigned long long)nq * (unsigned long long)((long long)a.cached[b] + tb + nq);
-  return (cost << 24) | (unsigned long long)(kEmMaxWork - 1 - i);
+// Adds, for the first N of a warp's tiles, the keys of this round that go before them.
+template <int N>
+__device__ __forceinline__ void em_count(const unsigned long long* keys, int n, int lane,
+                                         const unsigned long long (&mine)[kEmOwn], int (&before)[kEmOwn]) {
+#pragma unroll 4
+  for (int j = lane; j < n; j += 32) {
+    const unsigned long long x = keys[j];
+#pragma unroll
+    for (int m = 0; m < N; ++m) before[m] += x > mine[m];
+  }
 }
 
 __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMetaArgs a) {
   constexpr unsigned FULL = 0xffffffffu;
+  constexpr int NWARP = kEmThreads / 32;
   extern __shared__ __align__(16) uint8_t em_smem[];
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(em_smem);
-  int32_t* qo = reinterpret_cast<int32_t*>(em_smem + (size_t)kEmKeys * 8);  // [B + 1]
-  int32_t* kv = qo + a.B + 1;
-  int32_t* tl = kv + a.B + 1;
-  __shared__ long long wsum[3][kEmThreads / 32];
-  __shared__ int rank_of;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int B = a.B;
+  int32_t* qo = reinterpret_cast<int32_t*>(em_smem + (size_t)kEmKeys * 8);  // [B + 1] each
+  int32_t* kv = qo + B + 1;
+  int32_t* tl = kv + B + 1;
+  int32_t* cached = tl + B + 1;
+  int32_t* rows = cached + B + 1;  // -1: outside the table
+  __shared__ long long wsum[3][NWARP];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int P = 1 << a.page_log2;
 
   // ---- exclusive sums of new tokens, pages and tiles: thread t owns a run of requests
   {
     const int per = (B + kEmThreads - 1) / kEmThreads;
     const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
     long long s[3] = {0, 0, 0};
+    bool bad = false;
+#pragma unroll 4
     for (int b = b0; b < b1; ++b) {
-      const EmReq r = em_request(a, b);
-      const int tiles = (r.ext + a.tile_q - 1) / a.tile_q;
-      qo[b + 1] = r.ext;
-      kv[b + 1] = r.pages;
+      // lengths are forced into the table's range (and flagged)
+      const int L0 = a.lens[b], c0 = a.cached[b], r0 = a.rows[b];
+      const int L = L0 < 0 ? 0 : (int)min((int64_t)L0, a.stride);
+      const int c = min(max(c0, 0), L);
+      const bool row_ok = r0 >= 0 && r0 < a.table_rows;
+      bad = bad || L != L0 || c != c0 || !row_ok;
+      const int ext = L - c, pages = (int)(((int64_t)L + P - 1) >> a.page_log2);
+      const int tiles = (ext + a.tile_q - 1) / a.tile_q;
+      qo[b + 1] = ext;
+      kv[b + 1] = pages;
       tl[b + 1] = tiles;
-      s[0] += r.ext;
-      s[1] += r.pages;
+      cached[b] = c;
+      rows[b] = row_ok ? r0 : -1;
+      s[0] += ext;
+      s[1] += pages;
       s[2] += tiles;
     }
+    if (bad && blockIdx.x == 0) watchdog_set(kWdMetaOverflow);
     long long inc[3] = {s[0], s[1], s[2]};
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -143,7 +144,8 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
     for (int c = 0; c < 3; ++c) {
       base[c] = inc[c] - s[c];
       long long all = 0;
-      for (int w = 0; w < kEmThreads / 32; ++w) {
+#pragma unroll
+      for (int w = 0; w < NWARP; ++w) {
         if (w == warp) base[c] += all;
         all += wsum[c][w];
       }
@@ -165,7 +167,6 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
   }
   __syncthreads();
   const int T = qo[B], NP = kv[B], NT = tl[B];
-  const int P = 1 << a.page_log2;
   const int gthreads = gridDim.x * kEmThreads;
   const int gid = blockIdx.x * kEmThreads + tid;
 
@@ -176,8 +177,7 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
     if (b < B) {
       a.last_indices[b] = qo[b + 1] - 1;
       const int np = kv[b + 1] - kv[b];
-      const int L = a.cached[b] + (qo[b + 1] - qo[b]);
-      a.last_page_len[b] = np > 0 ? min(max(L - ((np - 1) << a.page_log2), 1), P) : 0;
+      a.last_page_len[b] = np > 0 ? cached[b] + (qo[b + 1] - qo[b]) - ((np - 1) << a.page_log2) : 0;
     }
   }
   if (gid == 0) {
@@ -188,32 +188,50 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
 
   // ---- positions and slots of the new tokens
   const int Tc = (int)min((int64_t)T, a.q_capacity);
-  for (int64_t i0 = (int64_t)gid * kEmVec; i0 < Tc; i0 += (int64_t)gthreads * kEmVec) {
-    int b = em_find(qo, B, (int)i0);
-    const int i1 = (int)min(i0 + kEmVec, (int64_t)Tc);
-    for (int i = (int)i0; i < i1; ++i) {
-      while (qo[b + 1] <= i) ++b;  // requests without new tokens
-      const int64_t row = a.rows[b];
-      const int pos = a.cached[b] + i - qo[b];
-      a.positions[i] = pos;
-      if (row >= 0 && row < a.table_rows && pos >= 0 && pos < a.stride) a.out_loc[i] = a.page_table[row * a.stride + pos];
+  for (int64_t i0 = gid; i0 < Tc; i0 += 4ll * gthreads) {
+    int pos[4], loc[4];
+    bool have[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = i0 + (int64_t)u * gthreads;
+      have[u] = i < Tc;
+      pos[u] = loc[u] = 0;
+      if (have[u]) {
+        const int b = em_find(qo, B, (int)i);
+        pos[u] = cached[b] + (int)i - qo[b];
+        have[u] = rows[b] >= 0;
+        if (have[u]) loc[u] = __ldg(a.page_table + (int64_t)rows[b] * a.stride + pos[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = i0 + (int64_t)u * gthreads;
+      if (i < Tc) a.positions[i] = pos[u];
+      if (have[u]) a.out_loc[i] = loc[u];
     }
   }
 
   // ---- page ids of every request's tokens
   const int NPc = (int)min((int64_t)NP, a.idx_capacity);
-  for (int64_t i0 = (int64_t)gid * kEmVec; i0 < NPc; i0 += (int64_t)gthreads * kEmVec) {
-    int b = em_find(kv, B, (int)i0);
-    const int i1 = (int)min(i0 + kEmVec, (int64_t)NPc);
-    for (int i = (int)i0; i < i1; ++i) {
-      while (kv[b + 1] <= i) ++b;  // requests without tokens
-      const int64_t row = a.rows[b];
-      const int64_t col = (int64_t)(i - kv[b]) << a.page_log2;
-      if (row >= 0 && row < a.table_rows && col < a.stride) {
-        const int32_t e = a.page_table[row * a.stride + col];
-        if (e < 0 || (e & (P - 1))) watchdog_set(kWdBadSlot);
-        a.kv_indices[i] = e >> a.page_log2;
+  for (int64_t i0 = gid; i0 < NPc; i0 += 4ll * gthreads) {
+    int e[4];
+    bool have[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = i0 + (int64_t)u * gthreads;
+      have[u] = i < NPc;
+      e[u] = 0;
+      if (have[u]) {
+        const int b = em_find(kv, B, (int)i);
+        have[u] = rows[b] >= 0;
+        if (have[u]) e[u] = __ldg(a.page_table + (int64_t)rows[b] * a.stride + ((int64_t)((int)i - kv[b]) << a.page_log2));
       }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (!have[u]) continue;
+      if (e[u] < 0 || (e[u] & (P - 1))) watchdog_set(kWdBadSlot);
+      a.kv_indices[i0 + (int64_t)u * gthreads] = e[u] >> a.page_log2;
     }
   }
 
@@ -221,38 +239,71 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
   for (int i = (NT > a.work_capacity ? 0 : NT) + gid; i < a.work_capacity; i += gthreads)
     reinterpret_cast<int4*>(a.work)[i] = make_int4(0, 0, 0, 0);
   if (NT > a.work_capacity) return;  // flagged above, the list stays empty
-  const int per = (NT + gridDim.x - 1) / gridDim.x;
-  const int o0 = min(blockIdx.x * per, NT), o1 = min(o0 + per, NT);
-  for (int own = o0; own < o1; ++own) {
-    const int b = em_find(tl, B, own);
-    int tb, nq;
-    const unsigned long long mine = em_key(a, qo, b, own - tl[b], own, tb, nq);
-    if (tid == 0) rank_of = 0;
-    int before = 0;
+  // key of tile i = tile k of request b: dearer tiles and, among equals, earlier ones are larger
+  auto tile_of = [&](int b, int i, int& tb, int& nq) -> unsigned long long {
+    tb = (i - tl[b]) * a.tile_q;
+    nq = min(a.tile_q, qo[b + 1] - qo[b] - tb);
+    const unsigned long long cost = (unsigned long long)nq * (unsigned long long)((long long)cached[b] + tb + nq);
+    return (cost << 24) | (unsigned long long)(kEmMaxWork - 1 - i);
+  };
+  const int per = (NT + (int)gridDim.x - 1) / (int)gridDim.x;
+  const int o0 = min((int)blockIdx.x * per, NT), o1 = min(o0 + per, NT);
+  for (int c0 = o0; c0 < o1; c0 += NWARP * kEmOwn) {
+    // this warp's tiles of the chunk: c0 + warp + 8 m
+    unsigned long long mine[kEmOwn];
+    int before[kEmOwn];
+#pragma unroll
+    for (int m = 0; m < kEmOwn; ++m) {
+      const int i = c0 + warp + NWARP * m;
+      int tb, nq;
+      before[m] = 0;
+      mine[m] = i < o1 ? tile_of(em_find(tl, B, i), i, tb, nq) : ~0ull;  // ~0: nothing goes before it
+    }
+    const int n_own = min(kEmOwn, (o1 - c0 - warp + NWARP - 1) / NWARP);
     for (int k0 = 0; k0 < NT; k0 += kEmKeys) {
       const int n = min(kEmKeys, NT - k0);
-      if (own == o0 || NT > kEmKeys) {  // one round serves every own tile when all keys fit
+      if (c0 == o0 || NT > kEmKeys) {  // one round's keys serve every chunk when they all fit
         __syncthreads();
         const int run = (n + kEmThreads - 1) / kEmThreads;
         const int j0 = min(tid * run, n), j1 = min(j0 + run, n);
         if (j0 < j1) {
-          int kb = em_find(tl, B, k0 + j0);
+          int b = em_find(tl, B, k0 + j0);
           for (int j = j0; j < j1; ++j) {
-            while (tl[kb + 1] <= k0 + j) ++kb;
-            int x, y;
-            keys[j] = em_key(a, qo, kb, k0 + j - tl[kb], k0 + j, x, y);
+            while (tl[b + 1] <= k0 + j) ++b;
+            int tb, nq;
+            keys[j] = tile_of(b, k0 + j, tb, nq);
           }
         }
+        __syncthreads();
       }
-      __syncthreads();
-      for (int j = tid; j < n; j += kEmThreads) before += keys[j] > mine;
+      switch (n_own) {  // uniform over the warp
+        case 1:
+          em_count<1>(keys, n, lane, mine, before);
+          break;
+        case 2:
+          em_count<2>(keys, n, lane, mine, before);
+          break;
+        case 3:
+          em_count<3>(keys, n, lane, mine, before);
+          break;
+        case 4:
+          em_count<4>(keys, n, lane, mine, before);
+          break;
+        default:
+          em_count<kEmOwn>(keys, n, lane, mine, before);
+      }
     }
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) before += __shfl_xor_sync(FULL, before, o);
-    if (lane == 0 && before) atomicAdd(&rank_of, before);
-    __syncthreads();
-    if (tid == 0) reinterpret_cast<int4*>(a.work)[rank_of] = make_int4(b, tb, nq, 0);
-    __syncthreads();
+    for (int m = 0; m < kEmOwn; ++m) {
+      const int rank = __reduce_add_sync(FULL, before[m]);
+      const int i = c0 + warp + NWARP * m;
+      if (lane == 0 && i < o1) {
+        const int b = em_find(tl, B, i);
+        int tb, nq;
+        tile_of(b, i, tb, nq);
+        reinterpret_cast<int4*>(a.work)[rank] = make_int4(b, tb, nq, 0);
+      }
+    }
   }
 }
 

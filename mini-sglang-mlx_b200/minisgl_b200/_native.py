@@ -161,10 +161,15 @@ def call(name: str, *args) -> None:
     """Call an int-status entry point and raise B200AttnError on failure."""
     rc = getattr(LIB, name)(*args)
     if rc != B2A_OK:
-        err = last_error()
-        if rc == B2A_ERR_INVALID:
-            raise ValueError(f"{name}: {err}")
-        raise B200AttnError(name, rc, err)
+        fail(name, rc)
+
+
+def fail(name: str, rc: int) -> None:
+    """Raise for a nonzero status of entry point ``name``."""
+    err = last_error()
+    if rc == B2A_ERR_INVALID:
+        raise ValueError(f"{name}: {err}")
+    raise B200AttnError(name, rc, err)
 
 
 def np_ptr(a: np.ndarray | None) -> int | None:

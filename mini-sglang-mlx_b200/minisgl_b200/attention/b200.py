@@ -16,6 +16,7 @@ backend refuses to construct.
 
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import List
 
@@ -24,8 +25,8 @@ import torch
 
 from .. import _native as nat
 from ..core import get_global_ctx
-from ..kvcache.fp4 import FP4KVCache, on_device
-from ..kvcache.pool import current_stream_ptr, dtype_code
+from ..kvcache.fp4 import FP4KVCache
+from ..kvcache.pool import current_stream_ptr, dtype_code, raw_stream
 from .base import CHECK_METADATA, BaseAttnBackend, PinnedStager, paged_kv_indices
 
 
@@ -83,6 +84,9 @@ class PackPlan:
     out_slots: int  # 16 n
 
 
+_NULL = nullcontext()
+
+
 def _page_size() -> int:
     try:
         return int(get_global_ctx().page_size)
@@ -116,6 +120,9 @@ class B200AttnBackend(BaseAttnBackend):
     @property
     def page_size(self) -> int:
         return self._page_size if self._page_size is not None else _page_size()
+
+    def _here(self):
+        return _NULL if torch.cuda.current_device() == self.device.index else torch.cuda.device(self.device)
 
     def _query(self, q: torch.Tensor) -> torch.Tensor:
         """q as the kernels read it: contiguous; over a 4-bit pool also of the cache's dtype and device."""
@@ -240,13 +247,13 @@ class B200AttnBackend(BaseAttnBackend):
         assert ws.numel() >= ws_bytes
         if self.fp4:
             kv = self.kv_cache
-            with on_device(self.device):
+            with self._here():
                 nat.call(
-                    "b2a_fp4_decode", q.data_ptr(), kv.rows(layer_id).data_ptr(), kv.num_tokens,
+                    "b2a_fp4_decode", q.data_ptr(), kv._base[layer_id], kv.num_tokens,
                     meta.kv_indices.data_ptr(), meta.page_size, meta.cta_indptr.data_ptr(), meta.segs.data_ptr(),
                     meta.num_ctas, meta.merge_indptr.data_ptr(), meta.n_partials, B, self.Hq, self.Hkv, self.D,
                     float(self.scale), kv.k_scale, kv.v_scale, ws.data_ptr(), ws.numel(), out.data_ptr(),
-                    self.dtype_code, current_stream_ptr(self.device),
+                    self.dtype_code, raw_stream(self.device.index),
                 )
             return out
         nat.call(
@@ -294,7 +301,7 @@ class B200AttnBackend(BaseAttnBackend):
         """Cut the keys of few work items into runs (4-bit pool): n_split and the batch's own workspace."""
         if not self.fp4:
             return
-        with on_device(self.device):
+        with self._here():
             meta.n_split = nat.fp4_extend_splits(meta.n_work, max_kv_len, self.Hq, self.Hkv, self.D, self.dtype_code)
             nbytes = int(nat.LIB.b2a_fp4_extend_workspace_bytes(meta.n_work, meta.n_split, self.Hkv, self.D))
             if nbytes:
@@ -355,14 +362,14 @@ class B200AttnBackend(BaseAttnBackend):
             if t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous() or t.device != self.device:
                 raise ValueError(f"{name} must be contiguous int32 [{B}] on {self.device}, got {t.dtype} "
                                  f"{tuple(t.shape)} on {t.device}")
-        with on_device(self.device):
+        with self._here():
             nat.call(
                 "b2a_extend_metadata", page_table.data_ptr(), page_table.shape[0], page_table.shape[1],
                 rows.data_ptr(), cached.data_ptr(), lens.data_ptr(), B, meta.page_size, meta.tile_q,
                 meta.qo_indptr.data_ptr(), meta.positions.data_ptr(), meta.out_loc.data_ptr(), meta.positions.numel(),
                 meta.last_indices.data_ptr(), meta.kv_indptr.data_ptr(), meta.kv_indices.data_ptr(),
                 meta.kv_indices.numel(), meta.kv_last_page_len.data_ptr(), meta.work.data_ptr(), meta.n_work,
-                meta.counts.data_ptr(), current_stream_ptr(self.device),
+                meta.counts.data_ptr(), raw_stream(self.device.index),
             )
 
     def _grouped_extend_metadata(self, qo_indptr, lens, src_indptr, src_indices, P, tile_q) -> B200PrefillMetadata:
@@ -406,15 +413,15 @@ class B200AttnBackend(BaseAttnBackend):
         B = meta.qo_indptr.numel() - 1
         if self.fp4:
             kv = self.kv_cache
-            with on_device(self.device):
+            with self._here():
                 nat.call(
-                    "b2a_fp4_extend", q.data_ptr(), kv.rows(layer_id).data_ptr(), kv.num_tokens,
+                    "b2a_fp4_extend", q.data_ptr(), kv._base[layer_id], kv.num_tokens,
                     meta.qo_indptr.data_ptr(), meta.kv_indptr.data_ptr(), meta.kv_indices.data_ptr(),
                     meta.kv_last_page_len.data_ptr(), meta.page_size, meta.work.data_ptr(), meta.n_work, meta.n_split,
                     T, B, self.Hq, self.Hkv, self.D, float(self.scale), kv.k_scale, kv.v_scale,
                     None if meta.workspace is None else meta.workspace.data_ptr(),
                     0 if meta.workspace is None else meta.workspace.numel(), out.data_ptr(), self.dtype_code,
-                    current_stream_ptr(self.device),
+                    raw_stream(self.device.index),
                 )
             return out
         k_pool, v_pool = self.kv_cache.k_cache(layer_id), self.kv_cache.v_cache(layer_id)

@@ -25,7 +25,7 @@ from contextlib import nullcontext
 import torch
 
 from .. import _native as nat
-from .pool import current_stream_ptr, dtype_code
+from .pool import dtype_code, raw_stream
 
 
 def on_device(device: torch.device):
@@ -48,7 +48,7 @@ class FP4KVCache:
         row = int(nat.LIB.b2a_fp4_row_bytes(num_kv_heads, head_dim))
         if row == 0:
             raise ValueError(f"FP4KVCache: {num_kv_heads} kv heads of {head_dim} features (64, 128 or 256) not supported")
-        dtype_code(dtype)
+        dtype_code(dtype)  # refuses a type the kernels do not take
         for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
             if not (s > 0 and 2.0 ** -100 <= s <= 2.0 ** 100 and float(s).hex().split("p")[0] == "0x1.0000000000000"):
                 raise ValueError(f"FP4KVCache: {name} must be a power of two in [2^-100, 2^100], got {s}")
@@ -70,54 +70,64 @@ class FP4KVCache:
         self.row_bytes = row
         self.k_scale = float(k_scale)
         self.v_scale = float(v_scale)
+        self._code = dtype_code(dtype)
+        self._base = [self.buffer[l].data_ptr() for l in range(num_layers)]
 
     def rows(self, layer_id: int) -> torch.Tensor:
         """uint8 ``[num_tokens, row_bytes]`` of a layer: the bytes the kernels read."""
         return self.buffer[layer_id]
 
-    def _slots(self, slots: torch.Tensor) -> None:
+    def _slots(self, slots: torch.Tensor) -> int:
         if slots.dtype != torch.int32 or slots.dim() != 1 or not slots.is_contiguous() or slots.device != self.device:
             raise ValueError(f"FP4KVCache: slots must be contiguous int32 [n] on {self.device}, got "
                              f"{slots.dtype} {tuple(slots.shape)} on {slots.device}")
+        return slots.shape[0]
+
+    def _rows(self, name: str, t: torch.Tensor, T: int) -> int:
+        """Element stride between the token rows of k or v ``[T, Hkv, D]``, checked."""
+        H, D = self.num_kv_heads, self.head_dim
+        if t.shape != (T, H, D) or t.dtype != self.dtype or t.device != self.device:
+            raise ValueError(f"FP4KVCache.store_kv: {name} must be {self.dtype} {(T, H, D)} on {self.device}, got "
+                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        row, head, elem = t.stride()
+        if T > 0 and (elem != 1 or (H > 1 and head != D)):
+            raise ValueError(f"FP4KVCache.store_kv: {name} rows must be [Hkv, D] contiguous")
+        return row if T > 1 else H * D
 
     def store_kv(self, k: torch.Tensor, v: torch.Tensor, out_loc: torch.Tensor, layer_id: int) -> None:
         """Quantise k/v ``[T, Hkv, D]`` into slots ``out_loc`` ``[T]`` (unique; token rows may be strided)."""
-        T = k.shape[0]
-        shape = (T, self.num_kv_heads, self.head_dim)
-        for name, t in (("k", k), ("v", v)):
-            if tuple(t.shape) != shape or t.dtype != self.dtype or t.device != self.device:
-                raise ValueError(f"FP4KVCache.store_kv: {name} must be {self.dtype} {shape} on {self.device}, got "
-                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
-            if T > 0 and (t.stride(2) != 1 or (shape[1] > 1 and t.stride(1) != shape[2])):
-                raise ValueError(f"FP4KVCache.store_kv: {name} rows must be [Hkv, D] contiguous")
-        self._slots(out_loc)
-        if out_loc.numel() != T:
-            raise ValueError(f"FP4KVCache.store_kv: {out_loc.numel()} slots for {T} tokens")
-        row = shape[1] * shape[2]
-        with on_device(self.device):
-            nat.call(
-                "b2a_fp4_store_kv", k.data_ptr(), k.stride(0) if T > 1 else row, v.data_ptr(),
-                v.stride(0) if T > 1 else row, out_loc.data_ptr(), self.buffer[layer_id].data_ptr(), self.num_tokens, T,
-                self.num_kv_heads, self.head_dim, self.k_scale, self.v_scale, dtype_code(self.dtype),
-                current_stream_ptr(self.device),
-            )
+        T = self._slots(out_loc)
+        ks, vs = self._rows("k", k, T), self._rows("v", v, T)
+        index = self.device.index
+        args = (k.data_ptr(), ks, v.data_ptr(), vs, out_loc.data_ptr(), self._base[layer_id], self.num_tokens, T,
+                self.num_kv_heads, self.head_dim, self.k_scale, self.v_scale, self._code, raw_stream(index))
+        if torch.cuda.current_device() == index:
+            rc = nat.LIB.b2a_fp4_store_kv(*args)
+        else:
+            with torch.cuda.device(index):
+                rc = nat.LIB.b2a_fp4_store_kv(*args)
+        if rc:
+            nat.fail("b2a_fp4_store_kv", rc)
 
     def load_kv(self, slots: torch.Tensor, layer_id: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The k and v ``[n, Hkv, D]`` that slots ``slots`` ``[n]`` of a layer stand for, in ``dtype``.
 
         Exact in fp32 and bf16. Rows of slots outside the pool are zero (and device error 32 is set).
         """
-        self._slots(slots)
-        n = slots.numel()
+        n = self._slots(slots)
         shape = (n, self.num_kv_heads, self.head_dim)
         k = torch.empty(shape, dtype=self.dtype, device=self.device)
         v = torch.empty(shape, dtype=self.dtype, device=self.device)
-        with on_device(self.device):
-            nat.call(
-                "b2a_fp4_load_kv", self.buffer[layer_id].data_ptr(), self.num_tokens, slots.data_ptr(), n,
-                self.num_kv_heads, self.head_dim, self.k_scale, self.v_scale, k.data_ptr(), v.data_ptr(),
-                dtype_code(self.dtype), current_stream_ptr(self.device),
-            )
+        index = self.device.index
+        args = (self._base[layer_id], self.num_tokens, slots.data_ptr(), n, self.num_kv_heads, self.head_dim,
+                self.k_scale, self.v_scale, k.data_ptr(), v.data_ptr(), self._code, raw_stream(index))
+        if torch.cuda.current_device() == index:
+            rc = nat.LIB.b2a_fp4_load_kv(*args)
+        else:
+            with torch.cuda.device(index):
+                rc = nat.LIB.b2a_fp4_load_kv(*args)
+        if rc:
+            nat.fail("b2a_fp4_load_kv", rc)
         return k, v
 
     @property

@@ -37,6 +37,12 @@ def current_stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# the raw cudaStream_t of a device's current stream, without building a Stream object (a
+# kernel launch of the 4-bit pool's small calls costs less than that object)
+raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class MHAKVCache:
     def __init__(
         self,
