@@ -421,23 +421,25 @@ int b2a_fp4_decode(const void* q, const void* pool, int64_t num_slots, const int
  * b2a_extend_plan or b2a_extend_metadata with the tile size that
  * b2a_fp4_extend_tile_q returns for the same shape; empty tiles at its end are
  * skipped. scale is positive and finite.
- * bf16 with D == 128 runs on tcgen05 tensor cores, where the keys of every work
- * item can be cut into n_split (at most 64) runs when there are few items:
- * b2a_fp4_extend_splits proposes a number for the longest request's length (1
- * for other shapes, which take only 1). With n_split > 1 the call needs a
- * 256-byte aligned workspace of b2a_fp4_extend_workspace_bytes: merge counters
- * (int32 [n_work * Hkv], zeroed once when it is allocated, zero again after every
- * call), then partial rows. One workspace serves calls that are ordered on the
- * GPU and have the same n_work and Hkv; it is not shared with b2a_fp4_decode.
+ * The keys of a work item can be cut into runs of run_keys keys (a multiple of
+ * 128), at most n_split (1 to 64) of them, the last one taking what is left:
+ * b2a_fp4_extend_runs (host only) proposes both for items whose last token sees
+ * tile_keys[i] keys (host array), n_split 1 when the items fill the GPU anyway.
+ * With n_split > 1 the call needs a 256-byte aligned workspace of
+ * b2a_fp4_extend_workspace_bytes: merge counters (int32 [n_work * Hkv], zeroed
+ * once when it is allocated, zero again after every call), then partial rows.
+ * One workspace serves calls that are ordered on the GPU and have the same
+ * n_work and Hkv; it is not shared with b2a_fp4_decode.
  * ------------------------------------------------------------------------ */
 int b2a_fp4_extend_tile_q(int Hq, int Hkv, int D, int dtype, int* tile_q);
-int b2a_fp4_extend_splits(int n_work, int64_t max_kv_len, int Hq, int Hkv, int D, int dtype, int* n_split);
+int b2a_fp4_extend_runs(const int32_t* tile_keys, int n_work, int Hq, int Hkv, int D, int dtype, int* run_keys,
+                        int* n_split);
 size_t b2a_fp4_extend_workspace_bytes(int n_work, int n_split, int Hkv, int D);
 int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int32_t* qo_indptr,
                    const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* kv_last_page_len, int page_size,
-                   const int32_t* work, int n_work, int n_split, int T, int B, int Hq, int Hkv, int D, float scale,
-                   float k_scale, float v_scale, void* workspace, size_t workspace_bytes, void* out, int dtype,
-                   void* stream);
+                   const int32_t* work, int n_work, int run_keys, int n_split, int T, int B, int Hq, int Hkv, int D,
+                   float scale, float k_scale, float v_scale, void* workspace, size_t workspace_bytes, void* out,
+                   int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
  * Prefill tables built on the device (stream-ordered, no host work, capturable

@@ -1299,43 +1299,41 @@ int b2a_fp4_decode(const void* q, const void* pool, int64_t num_slots, const int
 int b2a_fp4_extend_tile_q(int Hq, int Hkv, int D, int dtype, int* tile_q) {
   if (!tile_q) return fail(B2A_ERR_INVALID, "tile_q is NULL");
   if (int rc = fp4_extend_check(Hq, Hkv, D, dtype)) return rc;
-  const int G = Hq / Hkv;
-  *tile_q = b2a::extend_fp4_tc_supported(Hq, Hkv, D, dtype) ? b2a::extend_tc_tile_tokens(G) : b2a::kSimtRows / G;
+  *tile_q = b2a::extend_fp4_tile_tokens(Hq / Hkv, D, dtype == B2A_DTYPE_F32);
   return ok();
 }
 
-int b2a_fp4_extend_splits(int n_work, int64_t max_kv_len, int Hq, int Hkv, int D, int dtype, int* n_split) {
-  if (!n_split) return fail(B2A_ERR_INVALID, "n_split is NULL");
-  if (n_work < 0 || max_kv_len < 0) return fail(B2A_ERR_INVALID, "negative size");
+int b2a_fp4_extend_runs(const int32_t* tile_keys, int n_work, int Hq, int Hkv, int D, int dtype, int* run_keys,
+                        int* n_split) {
+  if (!run_keys || !n_split || (n_work > 0 && !tile_keys)) return fail(B2A_ERR_INVALID, "NULL argument");
+  if (n_work < 0) return fail(B2A_ERR_INVALID, "negative size");
   if (int rc = fp4_extend_check(Hq, Hkv, D, dtype)) return rc;
-  *n_split = 1;
-  if (n_work == 0 || !b2a::extend_fp4_tc_supported(Hq, Hkv, D, dtype)) return ok();
   const int sms = num_sms();
   if (sms <= 0) return fail(B2A_ERR_CUDA, "no CUDA device");
-  *n_split = b2a::extend_fp4_splits((int64_t)n_work * Hkv, sms, max_kv_len);
+  b2a::extend_fp4_runs(tile_keys, n_work, Hkv, sms, run_keys, n_split);
   return ok();
 }
 
 size_t b2a_fp4_extend_workspace_bytes(int n_work, int n_split, int Hkv, int D) {
   if (n_work <= 0 || n_split <= 1 || Hkv <= 0 || D <= 0) return 0;
   const size_t items = (size_t)n_work * Hkv;
-  return align256(items * sizeof(int32_t)) + items * n_split * 256 * (size_t)(D + 2) * sizeof(float);
+  return align256(items * sizeof(int32_t)) + items * n_split * b2a::kF4Rows * (size_t)(D + 2) * sizeof(float);
 }
 
 int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int32_t* qo_indptr,
                    const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* kv_last_page_len, int page_size,
-                   const int32_t* work, int n_work, int n_split, int T, int B, int Hq, int Hkv, int D, float scale,
-                   float k_scale, float v_scale, void* workspace, size_t workspace_bytes, void* out, int dtype,
-                   void* stream) {
+                   const int32_t* work, int n_work, int run_keys, int n_split, int T, int B, int Hq, int Hkv, int D,
+                   float scale, float k_scale, float v_scale, void* workspace, size_t workspace_bytes, void* out,
+                   int dtype, void* stream) {
   if (n_work < 0 || B < 0 || T < 0) return fail(B2A_ERR_INVALID, "negative size");
   if (int rc = fp4_extend_check(Hq, Hkv, D, dtype)) return rc;
   if (int rc = fp4_check(Hkv, D, k_scale, v_scale)) return rc;
   if (!(scale > 0.f) || scale > 1e30f) return fail(B2A_ERR_INVALID, "fp4 extend: scale must be positive and finite");
   const int plog = ilog2_exact(page_size);
   if (plog < 0) return fail(B2A_ERR_INVALID, "page_size %d must be a power of two", page_size);
-  const bool tc = b2a::extend_fp4_tc_supported(Hq, Hkv, D, dtype);
-  if (n_split < 1 || n_split > (tc ? 64 : 1))
-    return fail(B2A_ERR_INVALID, "fp4 extend: n_split %d out of [1, %d]", n_split, tc ? 64 : 1);
+  if (n_split < 1 || n_split > 64) return fail(B2A_ERR_INVALID, "fp4 extend: n_split %d out of [1, 64]", n_split);
+  if (n_split > 1 && (run_keys < 128 || run_keys % 128))
+    return fail(B2A_ERR_INVALID, "fp4 extend: run_keys %d must be a positive multiple of 128", run_keys);
   if (n_work == 0 || B == 0 || T == 0) return ok();
   if (!q || !pool || !qo_indptr || !kv_indptr || !kv_indices || !work || !out)
     return fail(B2A_ERR_INVALID, "NULL pointer argument");
@@ -1343,75 +1341,52 @@ int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int
   if (!aligned(q, 16) || !aligned(pool, 16) || !aligned(out, 16))
     return fail(B2A_ERR_INVALID, "q/pool/out must be 16-byte aligned");
   if (num_slots <= 0) return fail(B2A_ERR_INVALID, "num_slots must be > 0");
+  const size_t need = b2a_fp4_extend_workspace_bytes(n_work, n_split, Hkv, D);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(B2A_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  if (workspace && !aligned(workspace, 256)) return fail(B2A_ERR_INVALID, "workspace must be 256-byte aligned");
   const int G = Hq / Hkv;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (tc) {
-    const size_t need = b2a_fp4_extend_workspace_bytes(n_work, n_split, Hkv, D);
-    if (need > 0 && (!workspace || workspace_bytes < need))
-      return fail(B2A_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
-    if (workspace && !aligned(workspace, 256)) return fail(B2A_ERR_INVALID, "workspace must be 256-byte aligned");
-    b2a::F4Args a = {};
-    a.q = reinterpret_cast<const __nv_bfloat16*>(q);
-    a.pool = reinterpret_cast<const uint8_t*>(pool);
-    a.qo_indptr = qo_indptr;
-    a.kv_indptr = kv_indptr;
-    a.kv_indices = kv_indices;
-    a.kv_last_page_len = kv_last_page_len;
-    a.work = work;
-    a.out = reinterpret_cast<__nv_bfloat16*>(out);
-    if (need > 0) {
-      const size_t items = (size_t)n_work * Hkv;
-      a.tickets = reinterpret_cast<int32_t*>(workspace);
-      a.ws_acc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + align256(items * sizeof(int32_t)));
-      a.ws_ml = a.ws_acc + items * n_split * 256 * (size_t)D;
-    }
-    a.num_slots = num_slots;
-    a.row_bytes = b2a::fp4_row_bytes(Hkv, D);
-    a.page_log2 = plog;
-    a.Hq = Hq;
-    a.Hkv = Hkv;
-    a.G = G;
-    a.g_log2 = ilog2_exact(G);
-    a.n_split = n_split;
-    a.qscale = scale * k_scale * b2a::kLog2e;
-    a.v_scale = v_scale;
-    if (int rc = ensure_smem((const void*)b2a::extend_fp4_tc_kernel, b2a::F4Smem::ALLOC, "fp4_extend")) return rc;
-    // grid order as extend_tc.cuh: heads innermost, cost-sorted items behind them, runs outermost
-    for (int off = 0; off < n_work; off += 65535) {
-      a.item0 = off;
-      b2a::extend_fp4_tc_kernel<<<dim3(Hkv, std::min(65535, n_work - off), n_split), b2a::kF4Threads,
-                                  b2a::F4Smem::ALLOC, st>>>(a);
-    }
-    return check_launch("extend_fp4_tc_kernel");
-  }
-  b2a::ExtendArgs a = {};
+  b2a::F4Args a = {};
   a.q = q;
-  a.k_pool = pool;
+  a.pool = reinterpret_cast<const uint8_t*>(pool);
   a.qo_indptr = qo_indptr;
   a.kv_indptr = kv_indptr;
   a.kv_indices = kv_indices;
   a.kv_last_page_len = kv_last_page_len;
   a.work = work;
   a.out = out;
+  if (need > 0) {
+    const size_t items = (size_t)n_work * Hkv;
+    a.tickets = reinterpret_cast<int32_t*>(workspace);
+    a.ws_acc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + align256(items * sizeof(int32_t)));
+    a.ws_ml = a.ws_acc + items * n_split * b2a::kF4Rows * (size_t)D;
+  }
   a.num_slots = num_slots;
+  a.row_bytes = b2a::fp4_row_bytes(Hkv, D);
   a.page_log2 = plog;
   a.Hq = Hq;
   a.Hkv = Hkv;
+  a.G = G;
+  a.g_log2 = ilog2_exact(G);
+  a.n_split = n_split;
+  a.run_keys = run_keys;
   a.qscale = scale * k_scale * b2a::kLog2e;
-  a.row_bytes = (int)b2a::fp4_row_bytes(Hkv, D);
   a.v_scale = v_scale;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return with_dtype<false>(dtype, [&](auto tag) -> int {
-    using Tt = decltype(tag);
+    constexpr bool F32 = std::is_same<decltype(tag), float>::value;
     return with_d(D, [&](auto dc) -> int {
       constexpr int Dc = decltype(dc)::value;
-      return with_g<Dc>(G, [&](auto gc) -> int {
-        constexpr int Gc = decltype(gc)::value;
-        auto kern = b2a::extend_simt_kernel<Tt, Dc, Gc, true>;
-        const size_t smem = b2a::extend_simt_smem(Dc);
-        if (int rc = ensure_smem((const void*)kern, smem, "fp4_extend")) return rc;
-        kern<<<dim3(n_work, Hkv), b2a::kSimtThreads, smem, st>>>(a);
-        return check_launch("extend_simt_kernel (fp4)");
-      });
+      auto kern = b2a::extend_fp4_tc_kernel<Dc, F32>;
+      constexpr size_t smem = b2a::F4Cfg<Dc, F32>::ALLOC;
+      if (int rc = ensure_smem((const void*)kern, smem, "fp4_extend")) return rc;
+      // grid order as extend_tc.cuh: heads innermost, cost-sorted items behind them, runs outermost
+      for (int off = 0; off < n_work; off += 65535) {
+        b2a::F4Args b = a;
+        b.item0 = off;
+        kern<<<dim3(Hkv, std::min(65535, n_work - off), n_split), b2a::kF4Threads, smem, st>>>(b);
+      }
+      return check_launch("extend_fp4_tc_kernel");
     });
   });
 }

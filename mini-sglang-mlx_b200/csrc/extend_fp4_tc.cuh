@@ -1,27 +1,37 @@
 // Ragged causal extend attention over the 4-bit KV pool on tcgen05 tensor cores
-// (bf16 queries, head_dim 128, GQA group 1, 2, 4 or 8, any page size).
+// (bf16 or fp32 queries, head_dim 64, 128 or 256, GQA group 1, 2, 4 or 8, any page size).
 //
 //   O = softmax(scale * Q K^T, causal to the bottom right) V,   K, V of fp4_kv.cuh
 //
-// The tile, the MMA order, the softmax and the counted releases of P are those
-// of extend_tc.cuh (two 128-row tiles of one request and kv head share each block
-// of 128 keys; S and O in TMEM, one softmax thread per row, P written over S). What
-// differs is where K and V come from. A warpgroup of 128 threads expands the block:
-// thread i owns key i, reads its 64 + 64 code bytes and 16 scale bytes from the pool
-// (any slot: page ids are looked up per key, so every page size works and nothing is
-// staged), and writes the fp16 rows into the SWIZZLE_128B tiles the MMAs read. Loads
-// for block j + 1 are issued as soon as block j's registers are free, the page id of
-// block j + 2 with them, so the two dependent reads hide behind a block's time.
-// code * s is exact in fp16 (fp4_kv.cuh), and so is q after a power of two per row
-// (decode_fp4.cuh), undone in the row's softmax scale: the products are exact.
+// A 128-row tile packs 128 / G query tokens x the G heads of a kv head (extend_tc.cuh). A CTA
+// runs two streams (one at head_dim 256, whose accumulators fill TMEM), each with its own S, P
+// and O in TMEM and its own softmax warpgroup, one thread per row:
+//   wide    an item of more than one tile: stream t owns tile t, both read every key block
+//   narrow  an item of one tile: both streams own it, stream t reads the key blocks of parity t,
+//           and their (m, l, O) are joined at the end. One tile alone leaves the tensor cores
+//           idle while its softmax runs; measured on 8 requests of 1 to 16 new tokens and 6,000
+//           to 16,000 cached ones: 134 us with one stream, see the figures below for two.
+// MMA order: the PV product of a block, then the same stream's next S, so one stream's MMAs run
+// under the other's softmax. A commit covers every earlier MMA, so s_full of a stream's next
+// block also says that its PV has finished.
 //
-// Few rows on a long prefix leave most SMs idle, so the keys of a work item can be
-// cut into n_split runs of blocks (grid z). Each run writes its unnormalised rows
-// and (m, l) to a workspace; the CTA that takes the item's last ticket joins them, in
-// run order. Nothing waits for another CTA.
+// K and V come from a warpgroup that expands them: a thread owns a key (K and V of one row; at
+// 64 keys a block, K or V of it), reads its codes and scales from the pool (any slot: page ids
+// are looked up per key, nothing is staged) and writes fp16 rows into the SWIZZLE_128B tiles
+// that the MMAs read. Loads for the next block go out as soon as a block's registers are free,
+// and the page id of the one after with them, so both reads hide behind a block's time.
+// code * s is exact in fp16 (fp4_kv.cuh), and so is a bf16 q after a power of two per row
+// (decode_fp4.cuh), undone in the row's softmax scale: the products are exact. fp32 q and P are
+// split into two fp16 parts each (22 bits): S sums two products per step and PV two, over blocks
+// of 64 keys so that both parts of P find room beside S.
 //
-// Register split: 512 threads launch with 128 registers (65,536 in all); the softmax
-// warpgroups take 168 each, the expanding one 112, the issuer's 64: 512 x 128 again.
+// Few rows on long prefixes leave most SMs idle, so the keys of an item can be cut into runs of
+// run_blocks blocks (grid z). Each run writes its unnormalised rows and (m, l) to a workspace;
+// the CTA that takes the item's last ticket joins them, in run order. Nothing waits for another
+// CTA.
+//
+// Register split: 512 threads launch with 128 registers (65,536 in all); the softmax warpgroups
+// take 168 each, the expanding one 112, the issuer's 64: 512 x 128 again.
 #pragma once
 
 #include "decode_fp4.cuh"
@@ -31,60 +41,78 @@
 namespace b2a {
 
 constexpr int kF4Threads = 512;
+constexpr int kF4Rows = 256;  // partial rows of an item in the workspace (two tiles)
 
 struct F4Args {
-  const __nv_bfloat16* q;
+  const void* q;
   const uint8_t* pool;
   const int32_t* qo_indptr;
   const int32_t* kv_indptr;
   const int32_t* kv_indices;
   const int32_t* kv_last_page_len;
   const int32_t* work;
-  __nv_bfloat16* out;
-  float* ws_acc;     // [item][head][split][256 rows][128]
-  float* ws_ml;      // [item][head][split][256 rows][2]
+  void* out;
+  float* ws_acc;     // [item][head][run][256 rows][D]
+  float* ws_ml;      // [item][head][run][256 rows][2]
   int32_t* tickets;  // [item][head]
   int64_t num_slots;
   uint32_t row_bytes;
   int page_log2;
   int Hq, Hkv, G, g_log2;
-  int n_split;
-  int item0;  // index of this launch's first work item
+  int n_split;   // most runs of an item (grid z)
+  int run_keys;  // keys of a run
+  int item0;     // index of this launch's first work item
   float qscale;  // scale * k_scale * log2(e)
   float v_scale;
 };
 
-struct F4Smem {
-  static constexpr uint32_t Q0 = 0;
-  static constexpr uint32_t K0 = Q0 + 2 * kTcTileBytes;
-  static constexpr uint32_t V0 = K0 + 2 * kTcTileBytes;
-  static constexpr uint32_t BARS = V0 + 2 * kTcTileBytes;
-  // q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], mma_done, spare, p_full at 14
+template <int D, bool F32>
+struct F4Cfg {
+  static constexpr int KB = F32 ? 64 : 128;       // keys of a block
+  static constexpr int NS = D == 256 ? 1 : 2;     // streams
+  static constexpr int STAGES = D == 256 ? 1 : 2; // K and V tiles in flight
+  static constexpr bool WIDE = !F32 && D <= 128;  // items of two tiles
+  static constexpr uint32_t QTILE = 128u * D * 2u;
+  static constexpr uint32_t KTILE = (uint32_t)KB * D * 2u;
+  static constexpr int QTILES = (WIDE || F32) ? 2 : 1;  // two tiles, or the two parts of one
+  static constexpr uint32_t QHALF = 128u * 128u;        // bytes between 64-feature columns of a tile
+  static constexpr uint32_t KHALF = (uint32_t)KB * 128u;
+  static constexpr int O_COL = NS * 128;  // TMEM columns: S_t at 128 t, O_t behind them
+  static constexpr int PLO_COL = 64;      // fp32: low part of P beside S (64 columns)
+  static constexpr uint32_t K0 = QTILES * QTILE;
+  static constexpr uint32_t V0 = K0 + STAGES * KTILE;
+  static constexpr uint32_t BARS = V0 + STAGES * KTILE;
+  // q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], mma_done at 13, p_full at 14
   static constexpr int NBARS = 22;
   static constexpr uint32_t TMEM_SLOT = BARS + NBARS * 8;
   static constexpr uint32_t ABORT = TMEM_SLOT + 8;
   static constexpr uint32_t PCNT = ABORT + 8;
   static constexpr uint32_t LAST = PCNT + 32;
-  static constexpr uint32_t QFAC = LAST + 16;  // float [2][128]: softmax scale of each row
-  static constexpr uint32_t TOTAL = QFAC + 1024;
+  static constexpr uint32_t QFAC = LAST + 16;    // float [2][128]: softmax scale of each row
+  static constexpr uint32_t ML = QFAC + 1024;    // float2 [128]: (m, l) of stream 1 (narrow)
+  static constexpr uint32_t TOTAL = ML + 1024;
   static constexpr uint32_t ALLOC = TOTAL + 1024;
+  static_assert(ALLOC <= 232448, "tiles must fit in shared memory");
+  static_assert(NS == 1 || 128u * D * 4u <= K0 + STAGES * KTILE, "stream 1's rows are joined through the tiles' space");
 };
 
-// fp16 x fp16 -> fp32, M = 128, N = 128.
-__host__ __device__ constexpr uint32_t f4_idesc(bool b_mn_major) {
-  return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+// fp16 x fp16 -> fp32, M = 128, N = n.
+__host__ __device__ constexpr uint32_t f4_idesc(bool b_mn_major, int n) {
+  return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 64 code bytes and 8 scale bytes of one row -> 128 fp16 in row `row` of an SW128 tile.
-__device__ __forceinline__ void f4_expand_row(uint8_t* tile, int row, const uint4 (&c)[4], uint2 sc) {
+// Codes (D/2 bytes) and scales (D/16 bytes, packed in words) of one row -> D fp16 in row `row`
+// of a SWIZZLE_128B tile whose 64-feature columns lie `half` bytes apart.
+template <int D>
+__device__ __forceinline__ void f4_expand_row(uint8_t* tile, uint32_t half, int row, const uint4 (&c)[D / 32],
+                                              const uint32_t (&sc)[D / 64]) {
   const uint32_t base = (uint32_t)row * 128u;
   const uint32_t x = (uint32_t)(row & 7);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {  // 16 code bytes: two blocks of 16 features
-    const uint32_t two = ((q < 2 ? sc.x : sc.y) >> ((q & 1) * 16)) & 0xffffu;
-    const uint32_t s01 = fp4_scale2_to_h2(two);
+  for (int q = 0; q < D / 32; ++q) {  // 16 code bytes: two blocks of 16 features
+    const uint32_t s01 = fp4_scale2_to_h2((sc[q >> 1] >> ((q & 1) * 16)) & 0xffffu);
     const uint32_t s0 = __byte_perm(s01, 0, 0x1010), s1 = __byte_perm(s01, 0, 0x3232);
     const uint32_t w[4] = {c[q].x, c[q].y, c[q].z, c[q].w};
 #pragma unroll
@@ -95,40 +123,60 @@ __device__ __forceinline__ void f4_expand_row(uint8_t* tile, int row, const uint
 #pragma unroll
       for (int e = 0; e < 4; ++e) r[e] = h2_mul(r[e], s);
       const int chunk = 4 * q + i;  // 16-byte chunk (8 features) of the row
-      *reinterpret_cast<uint4*>(tile + (chunk >> 3) * kTcHalfBytes + base + (((uint32_t)(chunk & 7) ^ x) << 4)) =
+      *reinterpret_cast<uint4*>(tile + (chunk >> 3) * half + base + (((uint32_t)(chunk & 7) ^ x) << 4)) =
           make_uint4(r[0], r[1], r[2], r[3]);
     }
   }
 }
 
+// One K or V row's registers: codes and scales, zero for a NULL source.
+template <int D>
+struct F4Row {
+  uint4 c[D / 32];
+  uint32_t s[D / 64];
+  __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* scales) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) c[i] = codes ? reinterpret_cast<const uint4*>(codes)[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) s[i] = codes ? reinterpret_cast<const uint32_t*>(scales)[i] : 0u;
+  }
+};
+
+template <int D, bool F32>
 __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Args a) {
+  using C = F4Cfg<D, F32>;
+  using T = std::conditional_t<F32, float, __nv_bfloat16>;
+  constexpr int KB = C::KB;
+  constexpr unsigned FULL = 0xffffffffu;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F4Smem::BARS);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
   uint64_t* q_full = bars + 0;
   uint64_t* k_full = bars + 1;   // [2]
   uint64_t* k_empty = bars + 3;  // [2]
   uint64_t* v_full = bars + 5;   // [2]
   uint64_t* v_empty = bars + 7;  // [2]
-  uint64_t* s_full = bars + 9;   // [2] per tile
+  uint64_t* s_full = bars + 9;   // [2] per stream
   uint64_t* mma_done = bars + 13;
-  uint64_t* p_full = bars + 14;  // [tile * 4 + half]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + F4Smem::TMEM_SLOT);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + F4Smem::ABORT);
-  uint32_t* pcnt = reinterpret_cast<uint32_t*>(smem + F4Smem::PCNT);
-  volatile int* s_last = reinterpret_cast<volatile int*>(smem + F4Smem::LAST);
-  float* qfac = reinterpret_cast<float*>(smem + F4Smem::QFAC);
+  uint64_t* p_full = bars + 14;  // [stream * 4 + half]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TMEM_SLOT);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::ABORT);
+  uint32_t* pcnt = reinterpret_cast<uint32_t*>(smem + C::PCNT);
+  volatile int* s_last = reinterpret_cast<volatile int*>(smem + C::LAST);
+  float* qfac = reinterpret_cast<float*>(smem + C::QFAC);
+  float2* ml1 = reinterpret_cast<float2*>(smem + C::ML);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.G;
   const int TT = kTcRows >> a.g_log2;  // tokens per tile
   const int item = a.item0 + blockIdx.y;
   const int4 w = reinterpret_cast<const int4*>(a.work)[item];
-  const int nq = min(w.z, 2 * TT);
-  if (w.z > nq && threadIdx.x == 0) watchdog_set(kWdTileTooLarge);
+  const int nq = min(w.z, C::WIDE ? 2 * TT : TT);
   if (nq <= 0) return;  // unused entry behind a device-built work list
+  if (w.z > nq && threadIdx.x == 0) watchdog_set(kWdTileTooLarge);
   const int r = w.x, tb = w.y;
-  const int nq_t[2] = {min(nq, TT), max(0, nq - TT)};
+  const bool wide = C::WIDE && nq > TT;
+  const int nq_t[2] = {min(nq, TT), wide ? nq - TT : min(nq, TT)};  // tokens of each stream's tile
   const int h = blockIdx.x;
   const int P = 1 << a.page_log2;
   const int q0 = a.qo_indptr[r];
@@ -137,24 +185,30 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
   const int npages = a.kv_indptr[r + 1] - pbeg;
   const int Lkv = npages > 0 ? ((npages - 1) << a.page_log2) + (a.kv_last_page_len ? a.kv_last_page_len[r] : P) : 0;
   const int prefix = Lkv - Lq;
-  // blocks each tile needs, then this CTA's run of them: [b0, b0 + nb)
+  // key blocks of the item, and this CTA's run of them: [b0, b0 + nb)
+  const int nb_all = (max(0, min(Lkv, prefix + tb + nq)) + KB - 1) / KB;
+  const int run = max(1, a.run_keys / KB);
+  const int runs = a.n_split > 1 ? max(1, min(a.n_split, (nb_all + run - 1) / run)) : 1;
+  if ((int)blockIdx.z >= runs) return;
+  const int b0 = blockIdx.z * run;
+  const int nb = ((int)blockIdx.z == runs - 1 ? nb_all : b0 + run) - b0;
+  // blocks of each stream: wide, those its own rows need; narrow, every other one
   int nb_t[2];
-  for (int t = 0; t < 2; ++t) {
-    const int kv_end = nq_t[t] > 0 ? max(0, min(Lkv, prefix + tb + t * TT + nq_t[t])) : 0;
-    nb_t[t] = (kv_end + kTcKeys - 1) / kTcKeys;
+  if (wide) {
+    const int end0 = max(0, min(Lkv, prefix + tb + TT));  // tile 0 is full
+    nb_t[0] = max(0, min((end0 + KB - 1) / KB - b0, nb));
+    nb_t[1] = nb;
+  } else {
+    nb_t[0] = C::NS == 2 ? (nb + 1) >> 1 : nb;
+    nb_t[1] = C::NS == 2 ? nb >> 1 : 0;
   }
-  const int nb_all = max(nb_t[0], nb_t[1]);
-  const int b0 = (int)((int64_t)nb_all * blockIdx.z / a.n_split);
-  const int b1 = (int)((int64_t)nb_all * (blockIdx.z + 1) / a.n_split);
-  for (int t = 0; t < 2; ++t) nb_t[t] = max(0, min(nb_t[t], b1) - b0);
-  const int nb = max(nb_t[0], nb_t[1]);
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 4);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], 4);  // one arrive per expanding warp
+      mbar_init(&k_full[i], KB / 32);  // one arrive per expanding warp
       mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 4);
+      mbar_init(&v_full[i], KB / 32);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
       for (int c = 0; c < 2; ++c) mbar_init(&p_full[i * 4 + c], 4);  // one arrive per softmax warp
@@ -179,83 +233,94 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------------- MMA issuer
-      constexpr uint32_t idesc_qk = f4_idesc(false);
-      constexpr uint32_t idesc_pv = f4_idesc(true);
-      bool ok = tc_wait(q_full, 0, abort_flag);
+      constexpr uint32_t idesc_qk = f4_idesc(false, KB);
+      constexpr uint32_t idesc_pv = f4_idesc(true, D);
+      auto slot = [](int j) { return C::STAGES == 2 ? j & 1 : 0; };
+      auto phase = [](int j) { return (uint32_t)(C::STAGES == 2 ? j >> 1 : j) & 1u; };
       auto issue_s = [&](int t, int j) {
-        const uint32_t sQ = smem_u32(smem + F4Smem::Q0 + t * kTcTileBytes);
-        const uint32_t sK = smem_u32(smem + F4Smem::K0 + (j & 1) * kTcTileBytes);
+        const uint32_t sQ = smem_u32(smem + (wide ? t * C::QTILE : 0u));
+        const uint32_t sK = smem_u32(smem + C::K0 + slot(j) * C::KTILE);
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const uint64_t ad = sw128_desc(sQ + (kk >> 2) * kTcHalfBytes + (kk & 3) * 32, 16, 1024);
-          const uint64_t bd = sw128_desc(sK + (kk >> 2) * kTcHalfBytes + (kk & 3) * 32, 16, 1024);
-          tc_mma_f16(tmem + t * 128, ad, bd, idesc_qk, kk > 0 ? 1u : 0u);
+        for (int part = 0; part < (F32 ? 2 : 1); ++part) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t ad = sw128_desc(sQ + part * C::QTILE + (kk >> 2) * C::QHALF + (kk & 3) * 32, 16, 1024);
+            const uint64_t bd = sw128_desc(sK + (kk >> 2) * C::KHALF + (kk & 3) * 32, 16, 1024);
+            tc_mma_f16(tmem + t * 128, ad, bd, idesc_qk, (part > 0 || kk > 0) ? 1u : 0u);
+          }
         }
         tc_commit(&s_full[t]);
       };
-      auto p_done = [&](int idx, int j) -> bool {
+      // P of (stream, half) released by all 4 softmax warps: an acquire load of the release
+      // count instead of an mbarrier wait (extend_tc.cuh)
+      auto p_done = [&](int idx, int jl) -> bool {
         uint32_t v;
         asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(&pcnt[idx])) : "memory");
-        return v >= 4u * (uint32_t)(j + 1);
+        return v >= 4u * (uint32_t)(jl + 1);
       };
-      auto issue_pv = [&](int t, int j, int half) {
-        const uint32_t sV = smem_u32(smem + F4Smem::V0 + (j & 1) * kTcTileBytes);
+      auto issue_pv = [&](int t, int j, int jl, int half) {
+        const uint32_t sV = smem_u32(smem + C::V0 + slot(j) * C::KTILE);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int kk = half * 4 + q;
-          const uint64_t bd = sw128_desc(sV + kk * 2048, kTcHalfBytes, 1024);
-          tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, bd, idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+        for (int q = 0; q < KB / 32; ++q) {
+          const int kk = half * (KB / 32) + q;
+          const uint64_t bd = sw128_desc(sV + kk * 2048, C::KHALF, 1024);
+          tc_mma_f16_ts(tmem + C::O_COL + t * D, tmem + t * 128 + kk * 8, bd, idesc_pv, (jl > 0 || kk > 0) ? 1u : 0u);
+          if constexpr (F32) tc_mma_f16_ts(tmem + C::O_COL + t * D, tmem + t * 128 + C::PLO_COL + kk * 8, bd, idesc_pv, 1u);
         }
       };
-      if (ok && nb > 0) {
-        ok = tc_wait(&k_full[0], 0, abort_flag);
-        if (ok) {
-          tc_fence_after();
-          for (int t = 0; t < 2; ++t)
-            if (nb_t[t] > 0) issue_s(t, 0);
-          tc_commit(&k_empty[0]);
-        }
+      const bool alternate = C::NS == 2 && !wide;  // block j belongs to stream j & 1
+      const int lead = alternate ? 2 : 1;          // a stream's next block
+      bool ok = tc_wait(q_full, 0, abort_flag);
+      for (int j = 0; j < min(lead, nb) && ok; ++j) {
+        ok = tc_wait(&k_full[slot(j)], phase(j), abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        for (int t = 0; t < C::NS; ++t)
+          if (alternate ? t == j : nb_t[t] > 0) issue_s(t, j);
+        tc_commit(&k_empty[slot(j)]);
       }
       for (int j = 0; j < nb && ok; ++j) {
-        if (!tc_wait(&v_full[j & 1], (uint32_t)(j >> 1) & 1u, abort_flag)) {
+        if (!tc_wait(&v_full[slot(j)], phase(j), abort_flag)) {
           ok = false;
           break;
         }
-        const bool more = j + 1 < nb;
+        const int jn = j + lead;
         bool k_next = false;
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (j < nb_t[t]) {
-            if (p_done(t * 4 + 1, j)) {
+        for (int t = 0; t < C::NS && ok; ++t) {
+          if (alternate && t != (j & 1)) continue;
+          const int jl = alternate ? j >> 1 : j;
+          if (jl < nb_t[t]) {
+            if (p_done(t * 4 + 1, jl)) {
               tc_fence_after();
-              issue_pv(t, j, 0);
-              issue_pv(t, j, 1);
+              issue_pv(t, j, jl, 0);
+              issue_pv(t, j, jl, 1);
             } else {
               for (int half = 0; half < 2 && ok; ++half) {
-                if (!p_done(t * 4 + half, j) && !tc_wait(&p_full[t * 4 + half], (uint32_t)j & 1u, abort_flag)) {
+                if (!p_done(t * 4 + half, jl) && !tc_wait(&p_full[t * 4 + half], (uint32_t)jl & 1u, abort_flag)) {
                   ok = false;
                   break;
                 }
                 tc_fence_after();
-                issue_pv(t, j, half);
+                issue_pv(t, j, jl, half);
               }
             }
             if (!ok) break;
           }
-          if (more && j + 1 < nb_t[t]) {
+          if (jl + 1 < nb_t[t]) {
             if (!k_next) {
-              if (!tc_wait(&k_full[(j + 1) & 1], (uint32_t)((j + 1) >> 1) & 1u, abort_flag)) {
+              if (!tc_wait(&k_full[slot(jn)], phase(jn), abort_flag)) {
                 ok = false;
                 break;
               }
               tc_fence_after();
               k_next = true;
             }
-            issue_s(t, j + 1);
+            issue_s(t, jn);
           }
         }
         if (!ok) break;
-        tc_commit(&v_empty[j & 1]);
-        if (more) tc_commit(&k_empty[(j + 1) & 1]);
+        tc_commit(&v_empty[slot(j)]);
+        if (k_next) tc_commit(&k_empty[slot(jn)]);
       }
       // every MMA issued above has completed once mma_done fires (also on the abort path)
       tc_commit(mma_done);
@@ -264,125 +329,149 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
   } else if (warp >= 12) {
     // ---------------------------------------------------------------- expanding warpgroup
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-    constexpr unsigned FULL = 0xffffffffu;
-    const int row = threadIdx.x - 384;  // key of a block, and row of a query tile
-    const uint32_t code_off = fp4_code_off(h, kTcD), scale_off = fp4_scale_off(h, a.Hkv, kTcD);
-    // pool row of this thread's key of block j; NULL past the last key
+    const int th = threadIdx.x - 384;
+    const int row = th & (KB - 1);                      // key of a block
+    const bool do_k = KB == 128 || th < 64, do_v = KB == 128 || th >= 64;
+    const uint32_t code_off = fp4_code_off(h, D), scale_off = fp4_scale_off(h, a.Hkv, D);
     auto page_of = [&](int j) -> int {
-      const int key = (b0 + j) * kTcKeys + row;
+      const int key = (b0 + j) * KB + row;
       return j < nb && key < Lkv ? a.kv_indices[pbeg + (key >> a.page_log2)] : -1;
     };
+    // pool row of this thread's key of block j; NULL past the last key or for a bad page id,
+    // which is recorded and read as zeros
     auto row_of = [&](int j, int page) -> const uint8_t* {
-      const int key = (b0 + j) * kTcKeys + row;
+      const int key = (b0 + j) * KB + row;
       if (j >= nb || key >= Lkv) return nullptr;
-      const int64_t slot = (int64_t)page * P + (key & (P - 1));
-      if (page < 0 || slot >= a.num_slots) {
+      const int64_t sl = (int64_t)page * P + (key & (P - 1));
+      if (page < 0 || sl >= a.num_slots) {
         watchdog_set(kWdBadSlot);
-        return nullptr;  // the key reads as zeros
+        return nullptr;
       }
-      return a.pool + (size_t)slot * a.row_bytes;
+      return a.pool + (size_t)sl * a.row_bytes;
     };
-    auto load4 = [&](const uint8_t* p, uint4 (&c)[4]) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = p ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
-    };
-    uint4 kc[4], vc[4];
-    uint2 ks = make_uint2(0, 0), vs = make_uint2(0, 0);
+    F4Row<D> kr, vr;
+    auto load_k = [&](const uint8_t* p) { kr.load(p ? p + code_off : nullptr, p + scale_off); };
+    auto load_v = [&](const uint8_t* p) { vr.load(p ? p + code_off + D / 2 : nullptr, p + scale_off + D / 16); };
     const uint8_t* src = row_of(0, page_of(0));
-    load4(src ? src + code_off : nullptr, kc);
-    load4(src ? src + code_off + 64 : nullptr, vc);
-    if (src) {
-      ks = *reinterpret_cast<const uint2*>(src + scale_off);
-      vs = *reinterpret_cast<const uint2*>(src + scale_off + 8);
-    }
+    if (do_k) load_k(src);
+    if (do_v) load_v(src);
     int page_next = page_of(1);
-    // ---- Q: fp16 rows scaled by a power of two; rows past the tile are zero
+    // ---- Q: fp16 rows scaled by a power of two (two parts for fp32); rows past the tile are zero
 #pragma unroll 1
-    for (int t = 0; t < 2; ++t) {
-      const int tok = row >> a.g_log2, g = row & (G - 1);
-      uint8_t* tile = smem + F4Smem::Q0 + t * kTcTileBytes;
-      float f = 1.f, inv = 1.f;
+    for (int t = 0; t < (wide ? 2 : 1); ++t) {
+      const int tok = th >> a.g_log2, g = th & (G - 1);
+      uint8_t* tile = smem + t * C::QTILE;
       const bool have = tok < nq_t[t];
-      const uint4* qrow = reinterpret_cast<const uint4*>(a.q + ((size_t)(q0 + tb + t * TT + tok) * a.Hq + h * G + g) * kTcD);
-      float amax = 0.f;
+      const T* qrow = reinterpret_cast<const T*>(a.q) + ((size_t)(q0 + tb + t * TT + tok) * a.Hq + h * G + g) * D;
+      float amax = 0.f, f, inv;
       if (have) {
 #pragma unroll 4
-        for (int c = 0; c < 16; ++c) {
-          const uint4 v = qrow[c];
-          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        for (int c = 0; c < D / 8; ++c) {
+          float v[8];
+          load_vec<T, 8>(qrow + 8 * c, v);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(u[e] << 16)), fabsf(__uint_as_float(u[e] & 0xffff0000u))));
+          for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
         }
       }
       fp4_row_factor(amax, f, inv);
-      qfac[t * 128 + row] = inv * a.qscale;
+      qfac[t * 128 + th] = inv * a.qscale;
 #pragma unroll 4
-      for (int c = 0; c < 16; ++c) {
-        uint4 v = have ? qrow[c] : make_uint4(0, 0, 0, 0);
-        uint32_t u[4] = {v.x, v.y, v.z, v.w};
+      for (int c = 0; c < D / 8; ++c) {
+        float v[8];
+        if (have) {
+          load_vec<T, 8>(qrow + 8 * c, v);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          u[e] = pack_h2(__uint_as_float(u[e] << 16) * f, __uint_as_float(u[e] & 0xffff0000u) * f);
-        *reinterpret_cast<uint4*>(tile + (c >> 3) * kTcHalfBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
-            make_uint4(u[0], u[1], u[2], u[3]);
+          for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        }
+        uint32_t u[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x0 = v[2 * e] * f, x1 = v[2 * e + 1] * f;
+          u[e] = pack_h2(x0, x1);
+          if constexpr (F32) {
+            const float2 hi = h2_to_f2(u[e]);
+            lo[e] = pack_h2(x0 - hi.x, x1 - hi.y);
+          }
+        }
+        const uint32_t off = (c >> 3) * C::QHALF + th * 128 + (((c & 7) ^ (th & 7)) << 4);
+        *reinterpret_cast<uint4*>(tile + off) = make_uint4(u[0], u[1], u[2], u[3]);
+        if constexpr (F32) *reinterpret_cast<uint4*>(tile + C::QTILE + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
     fence_async_shared();
     __syncwarp();
     if (lane == 0) mbar_arrive(q_full);
     for (int j = 0; j < nb; ++j) {
-      const int st = j & 1;
-      const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-      if (!__all_sync(FULL, tc_wait(&k_empty[st], ph ^ 1u, abort_flag))) break;
-      f4_expand_row(smem + F4Smem::K0 + st * kTcTileBytes, row, kc, ks);
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&k_full[st]);
+      const int st = C::STAGES == 2 ? j & 1 : 0;
+      const uint32_t ph = (uint32_t)(C::STAGES == 2 ? j >> 1 : j) & 1u;
+      if (do_k) {
+        if (!__all_sync(FULL, tc_wait(&k_empty[st], ph ^ 1u, abort_flag))) break;
+        f4_expand_row<D>(smem + C::K0 + st * C::KTILE, C::KHALF, row, kr.c, kr.s);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&k_full[st]);
+      }
       // the next block's row: its page id was read a block ago
       src = row_of(j + 1, page_next);
       page_next = page_of(j + 2);
-      load4(src ? src + code_off : nullptr, kc);
-      ks = src ? *reinterpret_cast<const uint2*>(src + scale_off) : make_uint2(0, 0);
-      if (!__all_sync(FULL, tc_wait(&v_empty[st], ph ^ 1u, abort_flag))) break;
-      f4_expand_row(smem + F4Smem::V0 + st * kTcTileBytes, row, vc, vs);
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[st]);
-      load4(src ? src + code_off + 64 : nullptr, vc);
-      vs = src ? *reinterpret_cast<const uint2*>(src + scale_off + 8) : make_uint2(0, 0);
+      if (do_k) load_k(src);
+      if (do_v) {
+        if (!__all_sync(FULL, tc_wait(&v_empty[st], ph ^ 1u, abort_flag))) break;
+        f4_expand_row<D>(smem + C::V0 + st * C::KTILE, C::KHALF, row, vr.c, vr.s);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[st]);
+        load_v(src);
+      }
     }
   } else {
     // ---------------------------------------------------------------- softmax + epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-    constexpr unsigned FULL = 0xffffffffu;
-    const int t = (warp - 4) >> 2;              // tile of this warpgroup
+    const int t = (warp - 4) >> 2;              // stream of this warpgroup
     const int row = (threadIdx.x - 128) & 127;  // TMEM lane = tile row
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lane_off;
-    const uint32_t tO = tmem + 256 + t * 128 + lane_off;
+    const uint32_t tO = tmem + C::O_COL + t * D + lane_off;
+    const int tile = wide ? t : 0;
     const int tok = row >> a.g_log2;
-    const int lim_abs = min(prefix + tb + t * TT + tok, Lkv - 1);  // last visible key of this row
+    const bool live = tok < nq_t[t];
+    // a warp whose rows all lie past the tile only keeps the protocol going: its rows of P
+    // and O hold anything and are not read
+    const bool warp_live = (((warp & 3) * 32) >> a.g_log2) < nq_t[t];
+    const int lim_abs = min(prefix + tb + tile * TT + tok, Lkv - 1);  // last visible key of this row
     float m = kNegInf, l = 0.f;
     bool ok = true;
-    const int my_nb = nb_t[t];
+    const int my_nb = t < C::NS ? nb_t[t] : 0;
     float qscale = 0.f;
     if (my_nb > 0) {
       ok = __all_sync(FULL, tc_wait(q_full, 0, abort_flag));
-      qscale = qfac[t * 128 + row];
+      qscale = qfac[tile * 128 + row];
     }
-    for (int j = 0; j < my_nb && ok; ++j) {
-      ok = __all_sync(FULL, tc_wait(&s_full[t], (uint32_t)j & 1u, abort_flag));
+    for (int jl = 0; jl < my_nb && ok; ++jl) {
+      ok = __all_sync(FULL, tc_wait(&s_full[t], (uint32_t)jl & 1u, abort_flag));
       if (!ok) break;
       tc_fence_after();
-      const int limit = lim_abs - (b0 + j) * kTcKeys;  // columns 0..limit are visible
-      const bool full = limit >= kTcKeys - 1;
+      const int j = (C::NS == 2 && !wide) ? 2 * jl + t : jl;
+      if (!warp_live) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          for (int c = 0; c < 2; ++c) {
+            mbar_arrive(&p_full[t * 4 + c]);
+            asm volatile("red.release.cta.shared::cta.add.u32 [%0], 1;" ::"r"(smem_u32(&pcnt[t * 4 + c])) : "memory");
+          }
+        }
+        continue;
+      }
+      const int limit = lim_abs - (b0 + j) * KB;  // columns 0..limit are visible
+      const bool full = limit >= KB - 1;
       // pass 1: raw row max over the visible columns
       float mxs[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) mxs[i] = kNegInf;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int half = 0; half < KB / 64; ++half) {
         uint32_t ua[32], ub[32];
         tmem_ld32(tS + half * 64, ua);
         tmem_ld32(tS + half * 64 + 32, ub);
@@ -412,10 +501,10 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
         alpha = ex2_approx(m - m_blk);
         m = m_blk;
       }
-      // O_t is stable here: s_full for this block implies PV_t of the previous block finished
-      if (j > 0 && __any_sync(FULL, alpha != 1.f)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
+      // O_t is stable here: s_full for this block implies that the stream's last PV has finished
+      if (jl > 0 && __any_sync(FULL, alpha != 1.f)) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
           uint32_t u[32];
           tmem_ld32(tO + c * 32, u);
           tmem_wait_ld();
@@ -424,7 +513,7 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
           tmem_st32(tO + c * 32, u);
         }
       }
-      // pass 2: p = 2^(s * scale - m), packed to fp16 pairs over the first 64 columns of S.
+      // pass 2: p = 2^(s * scale - m), packed to fp16 pairs over the first columns of S.
       // A row that has seen no key yet (m = -inf) has every column masked below.
       const float msub = m == kNegInf ? 0.f : m;
       const uint64_t sc2 = f2(qscale, qscale);
@@ -434,10 +523,10 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
       tmem_ld32(tS, ua);
       tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < KB / 32; ++c) {
         uint32_t(&cur)[32] = (c & 1) ? ub : ua;
         uint32_t(&nxt)[32] = (c & 1) ? ua : ub;
-        if (c < 3) tmem_ld32(tS + (c + 1) * 32, nxt);
+        if (c < KB / 32 - 1) tmem_ld32(tS + (c + 1) * 32, nxt);
         uint32_t pk[16];
         float xv[32];
 #pragma unroll
@@ -456,73 +545,137 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
         }
         // P columns [16c, 16c+16): every S column below 32(c+1) has been read
         tmem_st16(tS + c * 16, pk);
-        if (c & 1) {
+        if constexpr (F32) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 hi = h2_to_f2(pk[i]);
+            pk[i] = pack_h2(xv[2 * i] - hi.x, xv[2 * i + 1] - hi.y);
+          }
+          tmem_st16(tS + C::PLO_COL + c * 16, pk);
+        }
+        if (KB == 64 || (c & 1)) {
           // release this half of P to the PV MMA while the rest is computed
+          const int half = KB == 64 ? c : c >> 1;
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&p_full[t * 4 + (c >> 1)]);
-            asm volatile("red.release.cta.shared::cta.add.u32 [%0], 1;" ::"r"(smem_u32(&pcnt[t * 4 + (c >> 1)])) : "memory");
+            // the arrive first, then the counted release (extend_tc.cuh)
+            mbar_arrive(&p_full[t * 4 + half]);
+            asm volatile("red.release.cta.shared::cta.add.u32 [%0], 1;" ::"r"(smem_u32(&pcnt[t * 4 + half])) : "memory");
           }
         }
-        if (c < 3) tmem_wait_ld();
+        if (c < KB / 32 - 1) tmem_wait_ld();
       }
       const uint64_t s01 = f2_add(f2_add(ps2[0], ps2[1]), f2_add(ps2[2], ps2[3]));
       float lo, hi;
       f2_split(s01, lo, hi);
       l = l * alpha + (lo + hi);
     }
-    // ---- epilogue: O_t / l -> bf16 rows, or the unnormalised rows of a split item
+    // ---- epilogue
     const bool got = __all_sync(FULL, mbar_wait(mma_done, 0, kWdExtendBar));
     tc_fence_after();
-    const int g = row & (G - 1);
-    const size_t part = ((size_t)item * a.Hkv + h) * a.n_split;  // first split of this item and head
-    if (a.n_split == 1) {
-      if (ok && got && nq_t[t] > 0) {
-        const float inv = l > 0.f ? a.v_scale / l : 0.f;
-        __nv_bfloat16* dst = a.out + ((size_t)(q0 + tb + t * TT + tok) * a.Hq + h * G + g) * kTcD;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t u[32];
-          if (my_nb > 0) {
+    ok = ok && got;
+    // narrow: stream 1's rows go through shared memory (the tiles are no longer read) to stream
+    // 0, which joins them with its own. 16-byte chunks are permuted by row against conflicts.
+    float4* exch = reinterpret_cast<float4*>(smem);
+    constexpr int CH = D / 4;  // chunks of a row
+    const bool join = C::NS == 2 && !wide;
+    float w0 = 1.f, w1 = 0.f;  // factors of the own and of stream 1's row
+    if (join) {
+      if (t == 1) {
+        const bool any = my_nb > 0 && warp_live && ok;
+        if (any) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t u[32];
             tmem_ld32(tO + c * 32, u);
             tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              exch[row * CH + ((c * 8 + i) ^ (row & (CH - 1) & 15))] =
+                  make_float4(__uint_as_float(u[4 * i]), __uint_as_float(u[4 * i + 1]), __uint_as_float(u[4 * i + 2]),
+                              __uint_as_float(u[4 * i + 3]));
+          }
+        }
+        ml1[row] = make_float2(any ? m : kNegInf, any ? l : 0.f);
+      }
+      named_bar_sync(1, 256);
+      if (t == 0) {
+        const float2 o = ml1[row];
+        if (o.x != kNegInf || o.y != o.y) {
+          if (m == kNegInf && l == l) {
+            w0 = 0.f;
+            w1 = 1.f;
+            m = o.x;
+            l = o.y;
           } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = 0u;
+            const float M = fmaxf(m, o.x);
+            w0 = exp2f(m - M);
+            w1 = exp2f(o.x - M);
+            l = l * w0 + o.y * w1;
+            m = M;
           }
-          uint32_t pk[16];
+        }
+      }
+    }
+    // 32 columns of this row: own accumulator (none without blocks) and stream 1's
+    auto columns = [&](int c, float (&v)[32]) {
+      uint32_t u[32];
+      if (my_nb > 0) {
+        tmem_ld32(tO + c * 32, u);
+        tmem_wait_ld();
+      } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(__uint_as_float(u[2 * i]) * inv, __uint_as_float(u[2 * i + 1]) * inv);
-          if (tok < nq_t[t]) {
-            uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
+        for (int i = 0; i < 32; ++i) u[i] = 0u;
+      }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d4[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
-          }
+      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
+      if (join && nb_t[1] > 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 x = exch[row * CH + ((c * 8 + i) ^ (row & (CH - 1) & 15))];
+          v[4 * i] = v[4 * i] * w0 + x.x * w1;
+          v[4 * i + 1] = v[4 * i + 1] * w0 + x.y * w1;
+          v[4 * i + 2] = v[4 * i + 2] * w0 + x.z * w1;
+          v[4 * i + 3] = v[4 * i + 3] * w0 + x.w * w1;
+        }
+      }
+    };
+    const int g = row & (G - 1);
+    const bool writer = t < C::NS && (t == 0 || wide);  // this warpgroup's rows are the item's
+    const size_t part = ((size_t)item * a.Hkv + h) * a.n_split;  // first run of this item and head
+    T* out = reinterpret_cast<T*>(a.out);
+    if (runs == 1) {
+      if (writer && ok && warp_live) {
+        const float inv = l > 0.f ? a.v_scale / l : (l == l ? 0.f : l);
+        T* dst = out + ((size_t)(q0 + tb + tile * TT + tok) * a.Hq + h * G + g) * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float v[32];
+          columns(c, v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] *= inv;
+          if (live) store_vec<T, 32>(dst + c * 32, v);
         }
       }
     } else {
-      const size_t mine = (part + blockIdx.z) * 256 + t * 128 + row;
-      if (my_nb > 0 && ok && got) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t u[32];
-          tmem_ld32(tO + c * 32, u);
-          tmem_wait_ld();
-          if (tok < nq_t[t]) {
-            uint4* d4 = reinterpret_cast<uint4*>(a.ws_acc + mine * kTcD + c * 32);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d4[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
-          }
+      const size_t mine = (part + blockIdx.z) * kF4Rows + tile * 128 + row;
+      if (writer && ok && warp_live) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float v[32];
+          columns(c, v);
+          if (live) store_vec<float, 32>(a.ws_acc + mine * D + c * 32, v);
         }
       }
-      if (tok < nq_t[t]) *reinterpret_cast<float2*>(a.ws_ml + mine * 2) = make_float2(l != l ? 0.f : (l > 0.f ? m : kNegInf), l);
+      if (writer && live)
+        *reinterpret_cast<float2*>(a.ws_ml + mine * 2) = make_float2(l != l ? 0.f : (l > 0.f && ok ? m : kNegInf), l);
       __threadfence();  // publish this row at GPU scope before the ticket
       named_bar_sync(1, 256);
       if (threadIdx.x == 128) {
         const int prev = atomicAdd(&a.tickets[(size_t)item * a.Hkv + h], 1);
-        const bool last = prev == a.n_split - 1;
+        const bool last = prev == runs - 1;
         if (last) a.tickets[(size_t)item * a.Hkv + h] = 0;  // re-armed for the next call
         *s_last = last ? 1 : 0;
       }
@@ -530,28 +683,33 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
       if (*s_last) {
         __threadfence();
         // one warp per row: its partials in run order, read through L2 (other SMs wrote them)
-        for (int i = warp - 4; i < 256; i += 8) {
+        constexpr int EPT = D / 32;
+        for (int i = warp - 4; i < (wide ? 256 : 128); i += 8) {
           const int tt = i >> 7, rr = i & 127, tk = rr >> a.g_log2;
           if (tk >= nq_t[tt]) continue;
-          float M = kNegInf, Ls = 0.f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int s = 0; s < a.n_split; ++s) {
-            const size_t pr = (part + s) * 256 + i;
+          float M = kNegInf, Ls = 0.f, acc[EPT];
+#pragma unroll
+          for (int e = 0; e < EPT; ++e) acc[e] = 0.f;
+          for (int s = 0; s < runs; ++s) {
+            const size_t pr = (part + s) * kF4Rows + i;
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + pr * 2));
             if (ml.x == kNegInf) continue;
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.ws_acc + pr * kTcD) + lane);
             const float Mn = fmaxf(M, ml.x);
             const float keep = M == kNegInf ? 0.f : exp2f(M - Mn), wgt = exp2f(ml.x - Mn);
             Ls = Ls * keep + ml.y * wgt;
-            acc.x = acc.x * keep + v.x * wgt;
-            acc.y = acc.y * keep + v.y * wgt;
-            acc.z = acc.z * keep + v.z * wgt;
-            acc.w = acc.w * keep + v.w * wgt;
+            const float2* src = reinterpret_cast<const float2*>(a.ws_acc + pr * D + lane * EPT);
+#pragma unroll
+            for (int e = 0; e < EPT / 2; ++e) {
+              const float2 v = __ldcg(src + e);
+              acc[2 * e] = acc[2 * e] * keep + v.x * wgt;
+              acc[2 * e + 1] = acc[2 * e + 1] * keep + v.y * wgt;
+            }
             M = Mn;
           }
           const float inv = Ls > 0.f ? a.v_scale / Ls : (Ls != Ls ? Ls : 0.f);
-          __nv_bfloat16* dst = a.out + ((size_t)(q0 + tb + tt * TT + tk) * a.Hq + h * G + (rr & (G - 1))) * kTcD;
-          reinterpret_cast<uint2*>(dst)[lane] = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+#pragma unroll
+          for (int e = 0; e < EPT; ++e) acc[e] *= inv;
+          store_vec<T, EPT>(out + ((size_t)(q0 + tb + tt * TT + tk) * a.Hq + h * G + (rr & (G - 1))) * D + lane * EPT, acc);
         }
       }
     }
@@ -564,18 +722,33 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
   }
 }
 
-}  // namespace b2a
+// ------------------------------------------------------------ host side
+// Query tokens per work item.
+inline int extend_fp4_tile_tokens(int G, int D, bool f32) { return (!f32 && D <= 128 ? 2 : 1) * (kTcRows / G); }
 
-namespace b2a {
-
-inline bool extend_fp4_tc_supported(int Hq, int Hkv, int D, int dtype) { return extend_tc_supported(Hq, Hkv, D, dtype); }
-
-// Runs of key blocks per work item: as many as fill the SMs once (one CTA per SM), while a
-// run keeps at least two blocks of keys.
-inline int extend_fp4_splits(int64_t ctas, int sms, int64_t max_kv) {
-  const int64_t fill = ctas > 0 ? sms / ctas : 1;
-  const int64_t runs = (max_kv + 2 * kTcKeys - 1) / (2 * kTcKeys);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({fill, runs, 64}));
+// Cuts the keys of few work items into runs so that the CTAs (items x heads x runs) fill the
+// SMs once: the shortest run of whole 128-key blocks, at least four of them, whose count of CTAs
+// fits. keys[i]: keys that item i's last token sees. Sets run_keys and the most runs of an item.
+inline void extend_fp4_runs(const int32_t* keys, int n_work, int Hkv, int sms, int* run_keys, int* n_split) {
+  *run_keys = 0;
+  *n_split = 1;
+  int64_t most = 0, total = 0;
+  for (int i = 0; i < n_work; ++i) {
+    const int64_t nb = std::max<int64_t>(1, ((int64_t)keys[i] + 127) / 128);
+    most = std::max(most, nb);
+    total += nb;
+  }
+  const int64_t slots = sms / std::max(1, Hkv);  // runs that fit at once
+  if (n_work <= 0 || slots <= n_work || most <= 4) return;
+  int64_t run = std::max<int64_t>({4, (total + slots - 1) / slots, (most + 63) / 64});
+  for (; run < most; ++run) {
+    int64_t n = 0;
+    for (int i = 0; i < n_work; ++i) n += (std::max<int64_t>(1, ((int64_t)keys[i] + 127) / 128) + run - 1) / run;
+    if (n <= slots) break;
+  }
+  if (run >= most) return;
+  *run_keys = (int)(run * 128);
+  *n_split = (int)((most + run - 1) / run);
 }
 
 }  // namespace b2a

@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
           em_count<4>(keys, n, lane, mine, before);
           break;
         default:
-          em_count<kEmOwn>(keys, n, lane, mine, before);
+          if (n_own > 4) em_count<kEmOwn>(keys, n, lane, mine, before);
       }
     }
 #pragma unroll

@@ -13,7 +13,6 @@
 // lane-per-key dot products are bank-conflict free).
 #pragma once
 #include "common.cuh"
-#include "fp4_kv.cuh"
 
 namespace b2a {
 
@@ -31,8 +30,6 @@ struct ExtendArgs {
   int page_log2;
   int Hq, Hkv;
   float qscale;  // scale * log2(e)
-  int row_bytes = 0;   // 4-bit pool: bytes of a token row (k_pool is the pool, v_pool unused)
-  float v_scale = 1.f;    // 4-bit pool: factor of the V values
 };
 
 constexpr int kSimtRows = 64;  // rows per CTA (TQ * G)
@@ -47,9 +44,7 @@ __device__ __forceinline__ int request_kv_len(const int32_t* kv_indptr, const in
   return ((np - 1) << page_log2) + last;
 }
 
-// FP4: the pool is the 4-bit one of fp4_kv.cuh (k_pool); its blocks are expanded as they
-// enter shared memory, everything behind that is the same.
-template <typename T, int D, int G, bool FP4 = false>
+template <typename T, int D, int G>
 __global__ void __launch_bounds__(kSimtThreads) extend_simt_kernel(const ExtendArgs a) {
   constexpr int EPT = D / 32;
   constexpr int RPW = kSimtRows / (kSimtThreads / 32);  // rows per warp (8)
@@ -101,45 +96,21 @@ __global__ void __launch_bounds__(kSimtThreads) extend_simt_kernel(const ExtendA
 
   for (int kb = 0; kb < kv_end; kb += BK) {
     __syncthreads();
-    if constexpr (FP4) {
-      // one block of 16 features of K or V per thread and step
-      for (int idx = tid; idx < BK * (D / 8); idx += kSimtThreads) {
-        const int j = idx / (D / 8), c = idx - j * (D / 8);
-        const int kind = c >= D / 16, blk = c - kind * (D / 16);
-        const int pos = kb + j;
-        const int64_t slot = pos < kv_end ? (int64_t)pages[pos >> a.page_log2] * P + (pos & (P - 1)) : -1;
-        if (pos < kv_end && (slot < 0 || slot >= a.num_slots)) watchdog_set(kWdBadSlot);
-        float x[16];
-        if (pos < kv_end && slot >= 0 && slot < a.num_slots) {
-          const uint8_t* row = reinterpret_cast<const uint8_t*>(a.k_pool) + (size_t)slot * a.row_bytes;
-          const uint2 w = *reinterpret_cast<const uint2*>(row + fp4_code_off(h, D) + kind * (D / 2) + blk * 8);
-          const uint32_t sb = row[fp4_scale_off(h, a.Hkv, D) + kind * (D / 16) + blk];
-          fp4_expand16(w, sb, x);
-        } else {
-#pragma unroll
-          for (int u = 0; u < 16; ++u) x[u] = 0.f;
-        }
-        float* dst = kind ? Vs + j * D + blk * 16 : Ks + j * (D + 1) + blk * 16;
-#pragma unroll
-        for (int u = 0; u < 16; ++u) dst[u] = x[u];
+    for (int idx = tid; idx < BK * (D / 2); idx += kSimtThreads) {
+      const int j = idx / (D / 2), c = idx - j * (D / 2);
+      const int pos = kb + j;
+      float k2[2] = {0.f, 0.f}, v2[2] = {0.f, 0.f};
+      const int64_t slot = pos < kv_end ? (int64_t)pages[pos >> a.page_log2] * P + (pos & (P - 1)) : -1;
+      if (pos < kv_end && (slot < 0 || slot >= a.num_slots)) watchdog_set(kWdBadSlot);
+      if (pos < kv_end && slot >= 0 && slot < a.num_slots) {
+        const size_t off = ((size_t)slot * a.Hkv + h) * D + 2 * c;
+        load_vec<T, 2>(kp + off, k2);
+        load_vec<T, 2>(vp + off, v2);
       }
-    } else {
-      for (int idx = tid; idx < BK * (D / 2); idx += kSimtThreads) {
-        const int j = idx / (D / 2), c = idx - j * (D / 2);
-        const int pos = kb + j;
-        float k2[2] = {0.f, 0.f}, v2[2] = {0.f, 0.f};
-        const int64_t slot = pos < kv_end ? (int64_t)pages[pos >> a.page_log2] * P + (pos & (P - 1)) : -1;
-        if (pos < kv_end && (slot < 0 || slot >= a.num_slots)) watchdog_set(kWdBadSlot);
-        if (pos < kv_end && slot >= 0 && slot < a.num_slots) {
-          const size_t off = ((size_t)slot * a.Hkv + h) * D + 2 * c;
-          load_vec<T, 2>(kp + off, k2);
-          load_vec<T, 2>(vp + off, v2);
-        }
-        Ks[j * (D + 1) + 2 * c] = k2[0];
-        Ks[j * (D + 1) + 2 * c + 1] = k2[1];
-        Vs[j * D + 2 * c] = v2[0];
-        Vs[j * D + 2 * c + 1] = v2[1];
-      }
+      Ks[j * (D + 1) + 2 * c] = k2[0];
+      Ks[j * (D + 1) + 2 * c + 1] = k2[1];
+      Vs[j * D + 2 * c] = v2[0];
+      Vs[j * D + 2 * c + 1] = v2[1];
     }
     __syncthreads();
 
@@ -203,8 +174,7 @@ __global__ void __launch_bounds__(kSimtThreads) extend_simt_kernel(const ExtendA
     const int row = row0 + i;
     const int tok = row / G, g = row - tok * G;
     if (tok < nq) {
-      float inv = lsum > 0.f ? 1.f / lsum : 0.f;
-      if constexpr (FP4) inv *= a.v_scale;
+      const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
       float o[EPT];
 #pragma unroll
       for (int e = 0; e < EPT; ++e) o[e] = acc[i][e] * inv;

@@ -113,10 +113,11 @@ SIGNATURES = {
     "b2a_fp4_extend_tile_q": (c_int, [c_int, c_int, c_int, c_int, ctypes.POINTER(c_int)]),
     "b2a_fp4_extend": (
         c_int,
-        [_P, _P, c_int64, _P, _P, _P, _P, c_int, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float,
-         c_float, _P, c_size_t, _P, c_int, _P],
+        [_P, _P, c_int64, _P, _P, _P, _P, c_int, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
+         c_float, c_float, _P, c_size_t, _P, c_int, _P],
     ),
-    "b2a_fp4_extend_splits": (c_int, [c_int, c_int64, c_int, c_int, c_int, c_int, ctypes.POINTER(c_int)]),
+    "b2a_fp4_extend_runs": (
+        c_int, [_P, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_int), ctypes.POINTER(c_int)]),
     "b2a_fp4_extend_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "b2a_extend_metadata": (
         c_int,
@@ -209,10 +210,12 @@ def fp4_extend_tile_q(Hq: int, Hkv: int, D: int, dtype_code: int) -> int:
     return t.value
 
 
-def fp4_extend_splits(n_work: int, max_kv_len: int, Hq: int, Hkv: int, D: int, dtype_code: int) -> int:
-    n = c_int(0)
-    call("b2a_fp4_extend_splits", n_work, max_kv_len, Hq, Hkv, D, dtype_code, ctypes.byref(n))
-    return n.value
+def fp4_extend_runs(tile_keys: np.ndarray, Hq: int, Hkv: int, D: int, dtype_code: int) -> tuple[int, int]:
+    """(run_keys, n_split) for work items whose last token sees ``tile_keys`` keys (b2a_fp4_extend_runs)."""
+    keys = np.ascontiguousarray(tile_keys, dtype=np.int32)
+    run, n = c_int(0), c_int(1)
+    call("b2a_fp4_extend_runs", np_ptr(keys), keys.size, Hq, Hkv, D, dtype_code, ctypes.byref(run), ctypes.byref(n))
+    return run.value, n.value
 
 
 def extend_plan(qo_indptr: np.ndarray, kv_indptr: np.ndarray, kv_last_page_len: np.ndarray | None,

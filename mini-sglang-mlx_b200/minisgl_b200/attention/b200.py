@@ -70,7 +70,8 @@ class B200PrefillMetadata:
     out_loc: torch.Tensor | None = None
     counts: torch.Tensor | None = None
     tile_q: int = 0
-    # 4-bit pool: runs the keys of a work item are cut into, and the workspace of their partial rows
+    # 4-bit pool: keys of a run of a work item, the most runs of one, the workspace of their partial rows
+    run_keys: int = 0
     n_split: int = 1
     workspace: torch.Tensor | None = None
 
@@ -294,15 +295,15 @@ class B200AttnBackend(BaseAttnBackend):
             kv_indices=dev[3], kv_last_page_len=dev[4], work=dev[5].view(-1, 4), n_work=int(work.shape[0]),
             total_q=int(qo_indptr[-1]), page_size=P,
         )
-        self._split_extend(meta, int(lens.max(initial=0)))
+        if self.fp4:
+            r = work[:, 0]
+            self._split_extend(meta, (lens - np.asarray(extend))[r] + work[:, 1] + work[:, 2])
         return meta
 
-    def _split_extend(self, meta: B200PrefillMetadata, max_kv_len: int) -> None:
-        """Cut the keys of few work items into runs (4-bit pool): n_split and the batch's own workspace."""
-        if not self.fp4:
-            return
+    def _split_extend(self, meta: B200PrefillMetadata, tile_keys: np.ndarray) -> None:
+        """Cut the keys of few work items into runs (4-bit pool), with a workspace of the batch's own."""
         with self._here():
-            meta.n_split = nat.fp4_extend_splits(meta.n_work, max_kv_len, self.Hq, self.Hkv, self.D, self.dtype_code)
+            meta.run_keys, meta.n_split = nat.fp4_extend_runs(tile_keys, self.Hq, self.Hkv, self.D, self.dtype_code)
             nbytes = int(nat.LIB.b2a_fp4_extend_workspace_bytes(meta.n_work, meta.n_split, self.Hkv, self.D))
             if nbytes:
                 meta.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
@@ -340,7 +341,9 @@ class B200AttnBackend(BaseAttnBackend):
             last_indices=last, q_offsets=[], qo_indptr=qo, kv_indptr=kv, kv_indices=idx, kv_last_page_len=lpl,
             work=work.view(-1, 4), n_work=n_work, total_q=total_q, page_size=P, positions=pos, out_loc=loc,
             counts=counts, tile_q=tile_q)
-        self._split_extend(meta, min(total_pages * P, self.page_table.shape[1]))
+        if self.fp4 and n_work:
+            # the lengths are known on the device only: as if every item saw an even share of the pages
+            self._split_extend(meta, np.full(n_work, min(total_pages * P // batch_size, self.page_table.shape[1])))
         return meta
 
     def build_extend_metadata_device(self, meta: B200PrefillMetadata, page_table: torch.Tensor, rows: torch.Tensor,
@@ -417,8 +420,8 @@ class B200AttnBackend(BaseAttnBackend):
                 nat.call(
                     "b2a_fp4_extend", q.data_ptr(), kv._base[layer_id], kv.num_tokens,
                     meta.qo_indptr.data_ptr(), meta.kv_indptr.data_ptr(), meta.kv_indices.data_ptr(),
-                    meta.kv_last_page_len.data_ptr(), meta.page_size, meta.work.data_ptr(), meta.n_work, meta.n_split,
-                    T, B, self.Hq, self.Hkv, self.D, float(self.scale), kv.k_scale, kv.v_scale,
+                    meta.kv_last_page_len.data_ptr(), meta.page_size, meta.work.data_ptr(), meta.n_work, meta.run_keys,
+                    meta.n_split, T, B, self.Hq, self.Hkv, self.D, float(self.scale), kv.k_scale, kv.v_scale,
                     None if meta.workspace is None else meta.workspace.data_ptr(),
                     0 if meta.workspace is None else meta.workspace.numel(), out.data_ptr(), self.dtype_code,
                     raw_stream(self.device.index),

@@ -113,17 +113,17 @@ def test_tile_sizes_and_refusals():
 
 
 def _extend(**kw):
-    a = dict(q=PTR, pool=PTR, slots=64, qo=PTR, kv=PTR, idx=PTR, lpl=PTR, P=16, work=PTR, nw=4, ns=1, T=9, B=2, Hq=16,
+    a = dict(q=PTR, pool=PTR, slots=64, qo=PTR, kv=PTR, idx=PTR, lpl=PTR, P=16, work=PTR, nw=4, rk=128, ns=1, T=9, B=2, Hq=16,
              Hkv=8, D=128, scale=0.1, gk=1.0, gv=1.0, ws=PTR, wsb=0, out=PTR, dt=1)
     a.update(kw)
     nat.call("b2a_fp4_extend", a["q"], a["pool"], a["slots"], a["qo"], a["kv"], a["idx"], a["lpl"], a["P"], a["work"],
-             a["nw"], a["ns"], a["T"], a["B"], a["Hq"], a["Hkv"], a["D"], a["scale"], a["gk"], a["gv"], a["ws"],
+             a["nw"], a["rk"], a["ns"], a["T"], a["B"], a["Hq"], a["Hkv"], a["D"], a["scale"], a["gk"], a["gv"], a["ws"],
              a["wsb"], a["out"], a["dt"], None)
 
 
 @pytest.mark.parametrize("kw", [dict(nw=-1), dict(T=-1), dict(B=-1), dict(Hq=24), dict(Hq=15), dict(D=96), dict(dt=2),
                                 dict(scale=0.0), dict(scale=float("nan")), dict(gk=0.3), dict(P=24), dict(ns=0),
-                                dict(ns=65), dict(ns=2, dt=0), dict(ns=2, D=64), dict(q=None), dict(pool=None),
+                                dict(ns=65), dict(ns=2, rk=0), dict(ns=2, rk=64), dict(ns=2, rk=200), dict(q=None), dict(pool=None),
                                 dict(qo=None), dict(kv=None), dict(idx=None), dict(work=None), dict(out=None),
                                 dict(work=PTR + 8), dict(q=PTR + 8), dict(slots=0), dict(ns=2),
                                 dict(ns=2, ws=None, wsb=1 << 40), dict(ns=2, ws=PTR + 16, wsb=1 << 40)])
