@@ -1340,7 +1340,7 @@ int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int
   if (!aligned(work, 16)) return fail(B2A_ERR_INVALID, "work must be 16-byte aligned (read as int4)");
   if (!aligned(q, 16) || !aligned(pool, 16) || !aligned(out, 16))
     return fail(B2A_ERR_INVALID, "q/pool/out must be 16-byte aligned");
-  if (num_slots <= 0) return fail(B2A_ERR_INVALID, "num_slots must be > 0");
+  if (num_slots <= 0 || num_slots > 0x7fffffffLL) return fail(B2A_ERR_INVALID, "num_slots must be in (0, 2^31)");
   const size_t need = b2a_fp4_extend_workspace_bytes(n_work, n_split, Hkv, D);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(B2A_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);

@@ -16,10 +16,10 @@
 // block also says that its PV has finished.
 //
 // K and V come from a warpgroup that expands them: a thread owns a key (K and V of one row; at
-// 64 keys a block, K or V of it), reads its codes and scales from the pool (any slot: page ids
-// are looked up per key, nothing is staged) and writes fp16 rows into the SWIZZLE_128B tiles
-// that the MMAs read. Loads for the next block go out as soon as a block's registers are free,
-// and the page id of the one after with them, so both reads hide behind a block's time.
+// 64 keys a block, K or V of it; page ids are looked up per key, so any page size works). Its
+// warp copies the raw rows of its keys to shared memory (cp.async), the thread takes its row
+// into registers and writes fp16 rows into the SWIZZLE_128B tiles that the MMAs read. The next
+// block's copies go out as soon as the registers hold this one.
 // code * s is exact in fp16 (fp4_kv.cuh), and so is a bf16 q after a power of two per row
 // (decode_fp4.cuh), undone in the row's softmax scale: the products are exact. fp32 q and P are
 // split into two fp16 parts each (22 bits): S sums two products per step and PV two, over blocks
@@ -68,9 +68,9 @@ struct F4Args {
 
 template <int D, bool F32>
 struct F4Cfg {
-  static constexpr int KB = F32 ? 64 : 128;       // keys of a block
+  static constexpr int KB = (F32 || D == 256) ? 64 : 128;  // keys of a block
   static constexpr int NS = D == 256 ? 1 : 2;     // streams
-  static constexpr int STAGES = D == 256 ? 1 : 2; // K and V tiles in flight
+  static constexpr int STAGES = (F32 && D == 256) ? 1 : 2;  // K and V tiles in flight
   static constexpr bool WIDE = !F32 && D <= 128;  // items of two tiles
   static constexpr uint32_t QTILE = 128u * D * 2u;
   static constexpr uint32_t KTILE = (uint32_t)KB * D * 2u;
@@ -81,7 +81,12 @@ struct F4Cfg {
   static constexpr int PLO_COL = 64;      // fp32: low part of P beside S (64 columns)
   static constexpr uint32_t K0 = QTILES * QTILE;
   static constexpr uint32_t V0 = K0 + STAGES * KTILE;
-  static constexpr uint32_t BARS = V0 + STAGES * KTILE;
+  // raw rows: code bytes of K and V (of one of them at 64 keys a block), then the scales
+  static constexpr int CODE_BYTES = KB == 128 ? D : D / 2;
+  static constexpr int SCALE_BYTES = CODE_BYTES / 8;
+  static constexpr uint32_t RAW_PITCH = CODE_BYTES + 16;  // 16-byte reads of 8 rows hit 32 banks
+  static constexpr uint32_t RAW = V0 + STAGES * KTILE;
+  static constexpr uint32_t BARS = RAW + 128 * RAW_PITCH;
   // q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], mma_done at 13, p_full at 14
   static constexpr int NBARS = 22;
   static constexpr uint32_t TMEM_SLOT = BARS + NBARS * 8;
@@ -101,13 +106,23 @@ __host__ __device__ constexpr uint32_t f4_idesc(bool b_mn_major, int n) {
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
+// Asynchronous copy of N (4, 8 or 16) bytes to shared memory; zeros when `have` is false.
+template <int N>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool have) {
+  const int n = have ? N : 0;
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+}
+
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Codes (D/2 bytes) and scales (D/16 bytes, packed in words) of one row -> D fp16 in row `row`
 // of a SWIZZLE_128B tile whose 64-feature columns lie `half` bytes apart.
 template <int D>
-__device__ __forceinline__ void f4_expand_row(uint8_t* tile, uint32_t half, int row, const uint4 (&c)[D / 32],
-                                              const uint32_t (&sc)[D / 64]) {
+__device__ __forceinline__ void f4_expand_row(uint8_t* tile, uint32_t half, int row, const uint4* c,
+                                              const uint32_t* sc) {
   const uint32_t base = (uint32_t)row * 128u;
   const uint32_t x = (uint32_t)(row & 7);
 #pragma unroll
@@ -128,19 +143,6 @@ __device__ __forceinline__ void f4_expand_row(uint8_t* tile, uint32_t half, int 
     }
   }
 }
-
-// One K or V row's registers: codes and scales, zero for a NULL source.
-template <int D>
-struct F4Row {
-  uint4 c[D / 32];
-  uint32_t s[D / 64];
-  __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* scales) {
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) c[i] = codes ? reinterpret_cast<const uint4*>(codes)[i] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) s[i] = codes ? reinterpret_cast<const uint32_t*>(scales)[i] : 0u;
-  }
-};
 
 template <int D, bool F32>
 __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Args a) {
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
   }
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 4);
+    mbar_init(q_full, 8);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], KB / 32);  // one arrive per expanding warp
       mbar_init(&k_empty[i], 1);
@@ -330,101 +332,77 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
     // ---------------------------------------------------------------- expanding warpgroup
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     const int th = threadIdx.x - 384;
-    const int row = th & (KB - 1);                      // key of a block
+    const int row = th & (KB - 1);  // key of a block
     const bool do_k = KB == 128 || th < 64, do_v = KB == 128 || th >= 64;
-    const uint32_t code_off = fp4_code_off(h, D), scale_off = fp4_scale_off(h, a.Hkv, D);
+    const uint32_t code_off = fp4_code_off(h, D) + (KB == 64 && do_v ? D / 2 : 0);
+    const uint32_t scale_off = fp4_scale_off(h, a.Hkv, D) + (KB == 64 && do_v ? D / 16 : 0);
+    // page id and pool slot of this lane's key of block j: -1 past the last key or for a bad
+    // page id, which is recorded and read as zeros
     auto page_of = [&](int j) -> int {
       const int key = (b0 + j) * KB + row;
       return j < nb && key < Lkv ? a.kv_indices[pbeg + (key >> a.page_log2)] : -1;
     };
-    // pool row of this thread's key of block j; NULL past the last key or for a bad page id,
-    // which is recorded and read as zeros
-    auto row_of = [&](int j, int page) -> const uint8_t* {
+    auto slot_of = [&](int j, int page) -> int {
       const int key = (b0 + j) * KB + row;
-      if (j >= nb || key >= Lkv) return nullptr;
+      if (j >= nb || key >= Lkv) return -1;
       const int64_t sl = (int64_t)page * P + (key & (P - 1));
       if (page < 0 || sl >= a.num_slots) {
         watchdog_set(kWdBadSlot);
-        return nullptr;
+        return -1;
       }
-      return a.pool + (size_t)sl * a.row_bytes;
+      return (int)sl;
     };
-    F4Row<D> kr, vr;
-    auto load_k = [&](const uint8_t* p) { kr.load(p ? p + code_off : nullptr, p + scale_off); };
-    auto load_v = [&](const uint8_t* p) { vr.load(p ? p + code_off + D / 2 : nullptr, p + scale_off + D / 16); };
-    const uint8_t* src = row_of(0, page_of(0));
-    if (do_k) load_k(src);
-    if (do_v) load_v(src);
+    // A warp copies the raw bytes of its own 32 keys: NCH lanes take the 16-byte chunks of one
+    // row, so a copy touches 32 / NCH rows instead of 32 (a lane loading its own row costs the
+    // load unit 32 lines per instruction: 342 against 281 us on the ragged batch of 32 requests).
+    constexpr int NCH = C::CODE_BYTES / 16;
+    uint8_t* raw = smem + C::RAW + (uint32_t)(th & ~31) * C::RAW_PITCH;
+    auto fetch = [&](int sl) {
+      const uint32_t dst = smem_u32(raw);
+#pragma unroll
+      for (int it = 0; it < NCH; ++it) {
+        const int rr = it * (32 / NCH) + lane / NCH, ch = lane % NCH;
+        const int s2 = __shfl_sync(FULL, sl, rr);
+        cp_async<16>(dst + rr * C::RAW_PITCH + ch * 16, a.pool + (size_t)max(s2, 0) * a.row_bytes + code_off + ch * 16, s2 >= 0);
+      }
+      cp_async<C::SCALE_BYTES>(dst + lane * C::RAW_PITCH + C::CODE_BYTES,
+                               a.pool + (size_t)max(sl, 0) * a.row_bytes + scale_off, sl >= 0);
+    };
+    fetch(slot_of(0, page_of(0)));
     int page_next = page_of(1);
-    // ---- Q: fp16 rows scaled by a power of two (two parts for fp32); rows past the tile are zero
-#pragma unroll 1
-    for (int t = 0; t < (wide ? 2 : 1); ++t) {
-      const int tok = th >> a.g_log2, g = th & (G - 1);
-      uint8_t* tile = smem + t * C::QTILE;
-      const bool have = tok < nq_t[t];
-      const T* qrow = reinterpret_cast<const T*>(a.q) + ((size_t)(q0 + tb + t * TT + tok) * a.Hq + h * G + g) * D;
-      float amax = 0.f, f, inv;
-      if (have) {
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          float v[8];
-          load_vec<T, 8>(qrow + 8 * c, v);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
-        }
-      }
-      fp4_row_factor(amax, f, inv);
-      qfac[t * 128 + th] = inv * a.qscale;
-#pragma unroll 4
-      for (int c = 0; c < D / 8; ++c) {
-        float v[8];
-        if (have) {
-          load_vec<T, 8>(qrow + 8 * c, v);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = 0.f;
-        }
-        uint32_t u[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x0 = v[2 * e] * f, x1 = v[2 * e + 1] * f;
-          u[e] = pack_h2(x0, x1);
-          if constexpr (F32) {
-            const float2 hi = h2_to_f2(u[e]);
-            lo[e] = pack_h2(x0 - hi.x, x1 - hi.y);
-          }
-        }
-        const uint32_t off = (c >> 3) * C::QHALF + th * 128 + (((c & 7) ^ (th & 7)) << 4);
-        *reinterpret_cast<uint4*>(tile + off) = make_uint4(u[0], u[1], u[2], u[3]);
-        if constexpr (F32) *reinterpret_cast<uint4*>(tile + C::QTILE + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-    }
-    fence_async_shared();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(q_full);
+    const uint8_t* mine = raw + lane * C::RAW_PITCH;
     for (int j = 0; j < nb; ++j) {
       const int st = C::STAGES == 2 ? j & 1 : 0;
       const uint32_t ph = (uint32_t)(C::STAGES == 2 ? j >> 1 : j) & 1u;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      uint4 code[NCH];
+      uint32_t sc[C::SCALE_BYTES / 4];
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) code[i] = reinterpret_cast<const uint4*>(mine)[i];
+#pragma unroll
+      for (int i = 0; i < C::SCALE_BYTES / 4; ++i) sc[i] = reinterpret_cast<const uint32_t*>(mine + C::CODE_BYTES)[i];
+      __syncwarp();
+      // the next block's rows travel while this one is expanded; its page ids were read a block ago
+      fetch(slot_of(j + 1, page_next));
+      page_next = page_of(j + 2);
       if (do_k) {
         if (!__all_sync(FULL, tc_wait(&k_empty[st], ph ^ 1u, abort_flag))) break;
-        f4_expand_row<D>(smem + C::K0 + st * C::KTILE, C::KHALF, row, kr.c, kr.s);
+        f4_expand_row<D>(smem + C::K0 + st * C::KTILE, C::KHALF, row, code, sc);
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_full[st]);
       }
-      // the next block's row: its page id was read a block ago
-      src = row_of(j + 1, page_next);
-      page_next = page_of(j + 2);
-      if (do_k) load_k(src);
       if (do_v) {
         if (!__all_sync(FULL, tc_wait(&v_empty[st], ph ^ 1u, abort_flag))) break;
-        f4_expand_row<D>(smem + C::V0 + st * C::KTILE, C::KHALF, row, vr.c, vr.s);
+        f4_expand_row<D>(smem + C::V0 + st * C::KTILE, C::KHALF, row, code + (KB == 128 ? D / 32 : 0),
+                         sc + (KB == 128 ? D / 64 : 0));
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_full[st]);
-        load_v(src);
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");  // never leave while own copies may still be landing
   } else {
     // ---------------------------------------------------------------- softmax + epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
@@ -440,6 +418,50 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
     // and O hold anything and are not read
     const bool warp_live = (((warp & 3) * 32) >> a.g_log2) < nq_t[t];
     const int lim_abs = min(prefix + tb + tile * TT + tok, Lkv - 1);  // last visible key of this row
+    // ---- Q: fp16 rows scaled by a power of two (two parts for fp32); rows past the tile are
+    // zero. D / 8 lanes take a row; wide, a warpgroup converts its own tile, else both share one.
+    {
+      constexpr int LPR = D / 8, RI = 32 / LPR;  // lanes of a row, rows of a step
+      const int rows = wide ? 32 : 16;
+      const int r0 = wide ? (warp & 3) * 32 : (warp - 4) * 16;
+      uint8_t* qt = smem + (wide ? t * C::QTILE : 0u);
+      const int ch = lane % LPR;
+#pragma unroll 4
+      for (int i = 0; i < rows; i += RI) {
+        const int rw = r0 + i + lane / LPR, tk = rw >> a.g_log2;
+        float v[8];
+        if (tk < nq_t[tile]) {
+          load_vec<T, 8>(reinterpret_cast<const T*>(a.q) +
+                             ((size_t)(q0 + tb + tile * TT + tk) * a.Hq + h * G + (rw & (G - 1))) * D + 8 * ch, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        }
+        float amax = 0.f, f, inv;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
+#pragma unroll
+        for (int o = LPR / 2; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, o));
+        fp4_row_factor(amax, f, inv);
+        if (ch == 0) qfac[tile * 128 + rw] = inv * a.qscale;
+        uint32_t u[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x0 = v[2 * e] * f, x1 = v[2 * e + 1] * f;
+          u[e] = pack_h2(x0, x1);
+          if constexpr (F32) {
+            const float2 hi = h2_to_f2(u[e]);
+            lo[e] = pack_h2(x0 - hi.x, x1 - hi.y);
+          }
+        }
+        const uint32_t off = (ch >> 3) * C::QHALF + rw * 128 + (((ch & 7) ^ (rw & 7)) << 4);
+        *reinterpret_cast<uint4*>(qt + off) = make_uint4(u[0], u[1], u[2], u[3]);
+        if constexpr (F32) *reinterpret_cast<uint4*>(qt + C::QTILE + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
     float m = kNegInf, l = 0.f;
     bool ok = true;
     const int my_nb = t < C::NS ? nb_t[t] : 0;
