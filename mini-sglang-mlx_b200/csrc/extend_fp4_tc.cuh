@@ -11,9 +11,9 @@
 //           and their (m, l, O) are joined at the end. One tile alone leaves the tensor cores
 //           idle while its softmax runs; measured on 8 requests of 1 to 16 new tokens and 6,000
 //           to 16,000 cached ones: 134 us with one stream, see the figures below for two.
-// MMA order: the PV product of a block, then the same stream's next S, so one stream's MMAs run
-// under the other's softmax. A commit covers every earlier MMA, so s_full of a stream's next
-// block also says that its PV has finished.
+// MMA order of a stream: the PV product of a block, then its next S, so one stream's MMAs run
+// under the other's softmax. A commit covers every earlier MMA of its thread, so s_full of a
+// stream's next block also says that its PV has finished.
 //
 // K and V come from a warpgroup that expands them: a thread owns a key (K and V of one row; at
 // 64 keys a block, K or V of it; page ids are looked up per key, so any page size works). Its
@@ -100,6 +100,42 @@ struct F4Cfg {
   static_assert(ALLOC <= 232448, "tiles must fit in shared memory");
   static_assert(NS == 1 || 128u * D * 4u <= K0 + STAGES * KTILE, "stream 1's rows are joined through the tiles' space");
 };
+
+// Whole-warp wait on an mbarrier phase: one try first, the abort flag and the bounded wait of
+// extend_tc.cuh only behind it (a wait whose phase is complete is on every role's critical path).
+__device__ __forceinline__ bool f4_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, tc_wait(bar, parity, abort_flag));
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// MMAs whose SWIZZLE_128B descriptors (sw128_desc) come as words: lo holds the address and the
+// LBO, hi the rest, which does not change. ACC: add to D.
+template <bool ACC>
+__device__ __forceinline__ void f4_mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "n"(ACC ? 1 : 0)
+      : "memory");
+}
+__device__ __forceinline__ void f4_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 
 // fp16 x fp16 -> fp32, M = 128, N = n.
 __host__ __device__ constexpr uint32_t f4_idesc(bool b_mn_major, int n) {
@@ -215,7 +251,7 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
       mbar_init(&s_full[i], 1);
       for (int c = 0; c < 2; ++c) mbar_init(&p_full[i * 4 + c], 4);  // one arrive per softmax warp
     }
-    mbar_init(mma_done, 1);
+    mbar_init(mma_done, wide ? 1 : C::NS);  // one arrive per issuer
     for (int i = 0; i < 8; ++i) pcnt[i] = 0;
     *abort_flag = 0;
     fence_mbar_init();
@@ -233,99 +269,129 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 || (warp == 2 && C::NS == 2 && !wide)) {
       // ---------------------------------------------------------------- MMA issuer
+      // The whole warp runs the loop and one elected lane issues, so addresses and descriptors
+      // stay warp-uniform.
+      // Narrow: a thread per stream. MMAs block their issuer while the tensor pipe is busy, so
+      // with one thread the waits of one stream would hold up the other's MMAs. Wide: one thread
+      // for both. Two fall into step on the blocks they share, and both softmax warpgroups then
+      // compete for the exponential units while the tensor cores idle (317 against 281 us on
+      // the ragged batch); one thread's fixed order keeps them half a block apart.
+      const int mine_t = warp >> 1;
       constexpr uint32_t idesc_qk = f4_idesc(false, KB);
       constexpr uint32_t idesc_pv = f4_idesc(true, D);
       auto slot = [](int j) { return C::STAGES == 2 ? j & 1 : 0; };
       auto phase = [](int j) { return (uint32_t)(C::STAGES == 2 ? j >> 1 : j) & 1u; };
-      auto issue_s = [&](int t, int j) {
-        const uint32_t sQ = smem_u32(smem + (wide ? t * C::QTILE : 0u));
-        const uint32_t sK = smem_u32(smem + C::K0 + slot(j) * C::KTILE);
-#pragma unroll
-        for (int part = 0; part < (F32 ? 2 : 1); ++part) {
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t ad = sw128_desc(sQ + part * C::QTILE + (kk >> 2) * C::QHALF + (kk & 3) * 32, 16, 1024);
-            const uint64_t bd = sw128_desc(sK + (kk >> 2) * C::KHALF + (kk & 3) * 32, 16, 1024);
-            tc_mma_f16(tmem + t * 128, ad, bd, idesc_qk, (part > 0 || kk > 0) ? 1u : 0u);
-          }
-        }
-        tc_commit(&s_full[t]);
+      auto k_ready = [&](int j) -> bool {
+        if (!f4_wait(&k_full[slot(j)], phase(j), abort_flag)) return false;
+        tc_fence_after();
+        return true;
       };
-      // P of (stream, half) released by all 4 softmax warps: an acquire load of the release
-      // count instead of an mbarrier wait (extend_tc.cuh)
+      const bool leader = elect_one();
+      constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // SBO, version, swizzle
+      const uint32_t base = (smem_u32(smem) & 0x3FFFFu) >> 4;
+      constexpr uint32_t lbo_k = (16u >> 4) << 16, lbo_v = (C::KHALF >> 4) << 16;
+      auto issue_s = [&](int t, int j) {
+        const uint32_t aq = base + ((wide ? t * C::QTILE : 0u) >> 4) + lbo_k;
+        const uint32_t bk = base + ((C::K0 + slot(j) * C::KTILE) >> 4) + lbo_k;
+        const uint32_t d = tmem + t * 128;
+        if (leader) {
+          f4_mma_ss<false>(d, aq, bk, desc_hi, idesc_qk);
+#pragma unroll
+          for (int kk = 1; kk < D / 16; ++kk)
+            f4_mma_ss<true>(d, aq + (((kk >> 2) * C::QHALF + (kk & 3) * 32) >> 4),
+                            bk + (((kk >> 2) * C::KHALF + (kk & 3) * 32) >> 4), desc_hi, idesc_qk);
+          if constexpr (F32) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              f4_mma_ss<true>(d, aq + ((C::QTILE + (kk >> 2) * C::QHALF + (kk & 3) * 32) >> 4),
+                              bk + (((kk >> 2) * C::KHALF + (kk & 3) * 32) >> 4), desc_hi, idesc_qk);
+          }
+          tc_commit(&s_full[t]);
+        }
+        __syncwarp();
+      };
+      // P of a half released by all 4 softmax warps: an acquire load of the release count
+      // instead of an mbarrier wait (extend_tc.cuh)
       auto p_done = [&](int idx, int jl) -> bool {
         uint32_t v;
         asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(&pcnt[idx])) : "memory");
-        return v >= 4u * (uint32_t)(jl + 1);
+        return __all_sync(FULL, v >= 4u * (uint32_t)(jl + 1));
       };
       auto issue_pv = [&](int t, int j, int jl, int half) {
-        const uint32_t sV = smem_u32(smem + C::V0 + slot(j) * C::KTILE);
+        const uint32_t bv = base + ((C::V0 + slot(j) * C::KTILE) >> 4) + lbo_v;
+        const uint32_t d = tmem + C::O_COL + t * D, p = tmem + t * 128;
+        if (leader) {
 #pragma unroll
-        for (int q = 0; q < KB / 32; ++q) {
-          const int kk = half * (KB / 32) + q;
-          const uint64_t bd = sw128_desc(sV + kk * 2048, C::KHALF, 1024);
-          tc_mma_f16_ts(tmem + C::O_COL + t * D, tmem + t * 128 + kk * 8, bd, idesc_pv, (jl > 0 || kk > 0) ? 1u : 0u);
-          if constexpr (F32) tc_mma_f16_ts(tmem + C::O_COL + t * D, tmem + t * 128 + C::PLO_COL + kk * 8, bd, idesc_pv, 1u);
+          for (int q = 0; q < KB / 32; ++q) {
+            const int kk = half * (KB / 32) + q;
+            f4_mma_ts(d, p + kk * 8, bv + kk * (2048 >> 4), desc_hi, idesc_pv, (jl > 0 || kk > 0) ? 1u : 0u);
+            if constexpr (F32) f4_mma_ts(d, p + C::PLO_COL + kk * 8, bv + kk * (2048 >> 4), desc_hi, idesc_pv, 1u);
+          }
         }
+        __syncwarp();
       };
-      const bool alternate = C::NS == 2 && !wide;  // block j belongs to stream j & 1
-      const int lead = alternate ? 2 : 1;          // a stream's next block
-      bool ok = tc_wait(q_full, 0, abort_flag);
-      for (int j = 0; j < min(lead, nb) && ok; ++j) {
-        ok = tc_wait(&k_full[slot(j)], phase(j), abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        for (int t = 0; t < C::NS; ++t)
-          if (alternate ? t == j : nb_t[t] > 0) issue_s(t, j);
-        tc_commit(&k_empty[slot(j)]);
-      }
-      for (int j = 0; j < nb && ok; ++j) {
-        if (!tc_wait(&v_full[slot(j)], phase(j), abort_flag)) {
-          ok = false;
-          break;
+      auto commit = [&](uint64_t* bar) {
+        if (leader) tc_commit(bar);
+        __syncwarp();
+      };
+      // the PV product of a stream's block jl, once its P is there
+      auto pv = [&](int t, int j, int jl) -> bool {
+        if (p_done(t * 4 + 1, jl)) {
+          tc_fence_after();
+          issue_pv(t, j, jl, 0);
+          issue_pv(t, j, jl, 1);
+          return true;
         }
-        const int jn = j + lead;
-        bool k_next = false;
-        for (int t = 0; t < C::NS && ok; ++t) {
-          if (alternate && t != (j & 1)) continue;
-          const int jl = alternate ? j >> 1 : j;
-          if (jl < nb_t[t]) {
-            if (p_done(t * 4 + 1, jl)) {
-              tc_fence_after();
-              issue_pv(t, j, jl, 0);
-              issue_pv(t, j, jl, 1);
-            } else {
-              for (int half = 0; half < 2 && ok; ++half) {
-                if (!p_done(t * 4 + half, jl) && !tc_wait(&p_full[t * 4 + half], (uint32_t)jl & 1u, abort_flag)) {
-                  ok = false;
-                  break;
-                }
-                tc_fence_after();
-                issue_pv(t, j, jl, half);
-              }
+        for (int half = 0; half < 2; ++half) {
+          if (!p_done(t * 4 + half, jl) && !f4_wait(&p_full[t * 4 + half], (uint32_t)jl & 1u, abort_flag)) return false;
+          tc_fence_after();
+          issue_pv(t, j, jl, half);
+        }
+        return true;
+      };
+      bool ok = f4_wait(q_full, 0, abort_flag);
+      if (wide) {
+        if (ok && nb > 0 && (ok = k_ready(0))) {
+          for (int t = 0; t < 2; ++t)
+            if (nb_t[t] > 0) issue_s(t, 0);
+          commit(&k_empty[0]);
+        }
+        for (int j = 0; j < nb && ok; ++j) {
+          ok = f4_wait(&v_full[slot(j)], phase(j), abort_flag);
+          bool k_next = false;
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (j < nb_t[t]) ok = pv(t, j, j);
+            if (ok && j + 1 < nb_t[t]) {
+              if (!k_next) ok = k_next = k_ready(j + 1);
+              if (ok) issue_s(t, j + 1);
             }
-            if (!ok) break;
           }
-          if (jl + 1 < nb_t[t]) {
-            if (!k_next) {
-              if (!tc_wait(&k_full[slot(jn)], phase(jn), abort_flag)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              k_next = true;
-            }
-            issue_s(t, jn);
+          if (!ok) break;
+          commit(&v_empty[slot(j)]);
+          if (k_next) commit(&k_empty[slot(j + 1)]);
+        }
+      } else {
+        // this stream's blocks: t, t + 2, .. of two streams, or all
+        const int t = mine_t, first = t, step = C::NS, mine = nb_t[t];
+        if (ok && mine > 0 && (ok = k_ready(first))) {
+          issue_s(t, first);
+          commit(&k_empty[slot(first)]);
+        }
+        for (int jl = 0; jl < mine && ok; ++jl) {
+          const int j = first + jl * step;
+          ok = f4_wait(&v_full[slot(j)], phase(j), abort_flag) && pv(t, j, jl);
+          if (!ok) break;
+          commit(&v_empty[slot(j)]);
+          if (jl + 1 < mine && (ok = k_ready(j + step))) {
+            issue_s(t, j + step);
+            commit(&k_empty[slot(j + step)]);
           }
         }
-        if (!ok) break;
-        tc_commit(&v_empty[slot(j)]);
-        if (k_next) tc_commit(&k_empty[slot(jn)]);
       }
       // every MMA issued above has completed once mma_done fires (also on the abort path)
-      tc_commit(mma_done);
+      commit(mma_done);
       mbar_wait(mma_done, 0, kWdExtendDrain);
     }
   } else if (warp >= 12) {
@@ -333,9 +399,9 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     const int th = threadIdx.x - 384;
     const int row = th & (KB - 1);  // key of a block
-    const bool do_k = KB == 128 || th < 64, do_v = KB == 128 || th >= 64;
-    const uint32_t code_off = fp4_code_off(h, D) + (KB == 64 && do_v ? D / 2 : 0);
-    const uint32_t scale_off = fp4_scale_off(h, a.Hkv, D) + (KB == 64 && do_v ? D / 16 : 0);
+    const bool do_k = KB == 128 || th < 64;  // at 64 keys a block: K or V of this key
+    const uint32_t code_off = fp4_code_off(h, D) + (do_k ? 0 : D / 2);
+    const uint32_t scale_off = fp4_scale_off(h, a.Hkv, D) + (do_k ? 0 : D / 16);
     // page id and pool slot of this lane's key of block j: -1 past the last key or for a bad
     // page id, which is recorded and read as zeros
     auto page_of = [&](int j) -> int {
@@ -368,38 +434,60 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
       cp_async<C::SCALE_BYTES>(dst + lane * C::RAW_PITCH + C::CODE_BYTES,
                                a.pool + (size_t)max(sl, 0) * a.row_bytes + scale_off, sl >= 0);
     };
-    fetch(slot_of(0, page_of(0)));
-    int page_next = page_of(1);
+    // One block's codes and scales of this thread's key, out of the raw rows; the next block's
+    // rows then travel while this one is expanded (their page ids were read a block ago).
     const uint8_t* mine = raw + lane * C::RAW_PITCH;
-    for (int j = 0; j < nb; ++j) {
-      const int st = C::STAGES == 2 ? j & 1 : 0;
-      const uint32_t ph = (uint32_t)(C::STAGES == 2 ? j >> 1 : j) & 1u;
+    uint4 code[NCH];
+    uint32_t sc[C::SCALE_BYTES / 4];
+    int page_next = page_of(1);
+    auto take = [&](int j) {
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
-      uint4 code[NCH];
-      uint32_t sc[C::SCALE_BYTES / 4];
 #pragma unroll
       for (int i = 0; i < NCH; ++i) code[i] = reinterpret_cast<const uint4*>(mine)[i];
 #pragma unroll
       for (int i = 0; i < C::SCALE_BYTES / 4; ++i) sc[i] = reinterpret_cast<const uint32_t*>(mine + C::CODE_BYTES)[i];
       __syncwarp();
-      // the next block's rows travel while this one is expanded; its page ids were read a block ago
       fetch(slot_of(j + 1, page_next));
       page_next = page_of(j + 2);
-      if (do_k) {
-        if (!__all_sync(FULL, tc_wait(&k_empty[st], ph ^ 1u, abort_flag))) break;
-        f4_expand_row<D>(smem + C::K0 + st * C::KTILE, C::KHALF, row, code, sc);
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&k_full[st]);
+    };
+    auto put = [&](int j, bool is_k, const uint4* c, const uint32_t* s2) -> bool {
+      const int st = C::STAGES == 2 ? j & 1 : 0;
+      const uint32_t ph = (uint32_t)(C::STAGES == 2 ? j >> 1 : j) & 1u;
+      if (!f4_wait(is_k ? &k_empty[st] : &v_empty[st], ph ^ 1u, abort_flag)) return false;
+      f4_expand_row<D>(smem + (is_k ? C::K0 : C::V0) + st * C::KTILE, C::KHALF, row, c, s2);
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(is_k ? &k_full[st] : &v_full[st]);
+      return true;
+    };
+    fetch(slot_of(0, page_of(0)));
+    if constexpr (KB == 128) {
+      // K one block ahead of V: a stream's next S needs its K right after the PV that frees V's
+      // tile, and V only after the softmax behind that S
+      constexpr int NV = D / 32, NVS = D / 64;
+      bool ok = true;
+      uint4 vc[NV];
+      uint32_t vs[NVS];
+      if (nb > 0) {
+        take(0);
+        ok = put(0, true, code, sc);
       }
-      if (do_v) {
-        if (!__all_sync(FULL, tc_wait(&v_empty[st], ph ^ 1u, abort_flag))) break;
-        f4_expand_row<D>(smem + C::V0 + st * C::KTILE, C::KHALF, row, code + (KB == 128 ? D / 32 : 0),
-                         sc + (KB == 128 ? D / 64 : 0));
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[st]);
+      for (int j = 0; j < nb && ok; ++j) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) vc[i] = code[NV + i];
+#pragma unroll
+        for (int i = 0; i < NVS; ++i) vs[i] = sc[NVS + i];
+        if (j + 1 < nb) {
+          take(j + 1);
+          ok = put(j + 1, true, code, sc);
+        }
+        if (ok) ok = put(j, false, vc, vs);
+      }
+    } else {
+      for (int j = 0; j < nb; ++j) {
+        take(j);
+        if (!put(j, do_k, code, sc)) break;
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");  // never leave while own copies may still be landing
@@ -426,16 +514,36 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
       const int r0 = wide ? (warp & 3) * 32 : (warp - 4) * 16;
       uint8_t* qt = smem + (wide ? t * C::QTILE : 0u);
       const int ch = lane % LPR;
-#pragma unroll 4
-      for (int i = 0; i < rows; i += RI) {
-        const int rw = r0 + i + lane / LPR, tk = rw >> a.g_log2;
-        float v[8];
-        if (tk < nq_t[tile]) {
-          load_vec<T, 8>(reinterpret_cast<const T*>(a.q) +
-                             ((size_t)(q0 + tb + tile * TT + tk) * a.Hq + h * G + (rw & (G - 1))) * D + 8 * ch, v);
-        } else {
+      constexpr int GI = RI >= 4 ? 16 / RI : 8;  // steps whose loads go out together
+      constexpr int EV = F32 ? 2 : 1;             // 16-byte words of a lane's eight elements
+#pragma unroll 1
+      for (int i0 = 0; i0 < rows; i0 += GI * RI) {
+        uint4 raw[GI][EV];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        for (int i = 0; i < GI; ++i) {
+          const int rw = r0 + i0 + i * RI + lane / LPR, tk = rw >> a.g_log2;
+          const T* src = reinterpret_cast<const T*>(a.q) +
+                         ((size_t)(q0 + tb + tile * TT + tk) * a.Hq + h * G + (rw & (G - 1))) * D + 8 * ch;
+#pragma unroll
+          for (int e = 0; e < EV; ++e)
+            raw[i][e] = tk < nq_t[tile] ? reinterpret_cast<const uint4*>(src)[e] : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < GI; ++i) {
+        const int rw = r0 + i0 + i * RI + lane / LPR;
+        float v[8];
+        if constexpr (F32) {
+          const uint4 x = raw[i][0], y = raw[i][EV - 1];
+          const uint32_t w8[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w8[e]);
+        } else {
+          const uint32_t w4[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[2 * e] = __uint_as_float(w4[e] << 16);
+            v[2 * e + 1] = __uint_as_float(w4[e] & 0xffff0000u);
+          }
         }
         float amax = 0.f, f, inv;
 #pragma unroll
@@ -457,6 +565,7 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
         const uint32_t off = (ch >> 3) * C::QHALF + rw * 128 + (((ch & 7) ^ (rw & 7)) << 4);
         *reinterpret_cast<uint4*>(qt + off) = make_uint4(u[0], u[1], u[2], u[3]);
         if constexpr (F32) *reinterpret_cast<uint4*>(qt + C::QTILE + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
       }
       fence_async_shared();
       __syncwarp();
@@ -467,11 +576,11 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
     const int my_nb = t < C::NS ? nb_t[t] : 0;
     float qscale = 0.f;
     if (my_nb > 0) {
-      ok = __all_sync(FULL, tc_wait(q_full, 0, abort_flag));
+      ok = f4_wait(q_full, 0, abort_flag);
       qscale = qfac[tile * 128 + row];
     }
     for (int jl = 0; jl < my_nb && ok; ++jl) {
-      ok = __all_sync(FULL, tc_wait(&s_full[t], (uint32_t)jl & 1u, abort_flag));
+      ok = f4_wait(&s_full[t], (uint32_t)jl & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
       const int j = (C::NS == 2 && !wide) ? 2 * jl + t : jl;
