@@ -98,7 +98,9 @@ struct F4Cfg {
   static constexpr uint32_t TOTAL = ML + 1024;
   static constexpr uint32_t ALLOC = TOTAL + 1024;
   static_assert(ALLOC <= 232448, "tiles must fit in shared memory");
-  static_assert(NS == 1 || 128u * D * 4u <= K0 + STAGES * KTILE, "stream 1's rows are joined through the tiles' space");
+  // after the last MMA: stream 1's fp32 rows pass through the Q tiles, output rows through K and V
+  static_assert(NS == 1 || 128u * D * 4u <= K0, "stream 1's rows must fit in the Q tiles");
+  static_assert(NS == 1 || (WIDE ? 2u : 1u) * 128u * D * (F32 ? 4u : 2u) <= 2u * STAGES * KTILE, "output rows must fit");
 };
 
 // Whole-warp wait on an mbarrier phase: one try first, the abort flag and the bounded wait of
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
       const int r0 = wide ? (warp & 3) * 32 : (warp - 4) * 16;
       uint8_t* qt = smem + (wide ? t * C::QTILE : 0u);
       const int ch = lane % LPR;
-      constexpr int GI = RI >= 4 ? 16 / RI : 8;  // steps whose loads go out together
+      constexpr int GI = F32 || RI == 1 ? 8 : (C::WIDE && RI == 2 ? 16 : 16 / RI);  // steps whose loads go out together
       constexpr int EV = F32 ? 2 : 1;             // 16-byte words of a lane's eight elements
 #pragma unroll 1
       for (int i0 = 0; i0 < rows; i0 += GI * RI) {
@@ -526,30 +528,38 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
                          ((size_t)(q0 + tb + tile * TT + tk) * a.Hq + h * G + (rw & (G - 1))) * D + 8 * ch;
 #pragma unroll
           for (int e = 0; e < EV; ++e)
-            raw[i][e] = tk < nq_t[tile] ? reinterpret_cast<const uint4*>(src)[e] : make_uint4(0, 0, 0, 0);
+            raw[i][e] = i0 + i * RI < rows && tk < nq_t[tile] ? reinterpret_cast<const uint4*>(src)[e] : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < GI; ++i) {
+        if (i0 + i * RI >= rows) break;  // the next warp's rows
         const int rw = r0 + i0 + i * RI + lane / LPR;
-        float v[8];
+        float v[8], amax, f, inv;
         if constexpr (F32) {
           const uint4 x = raw[i][0], y = raw[i][EV - 1];
           const uint32_t w8[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          amax = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w8[e]);
+          for (int e = 0; e < 8; ++e) {
+            v[e] = __uint_as_float(w8[e]);
+            amax = fmaxf(amax, fabsf(v[e]));
+          }
+#pragma unroll
+          for (int o = LPR / 2; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, o));
         } else {
           const uint32_t w4[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
+          // non-negative bf16 pairs order like their bits
+          uint32_t mx = __vmaxu2(__vmaxu2(w4[0] & 0x7fff7fffu, w4[1] & 0x7fff7fffu),
+                                 __vmaxu2(w4[2] & 0x7fff7fffu, w4[3] & 0x7fff7fffu));
+#pragma unroll
+          for (int o = LPR / 2; o >= 1; o >>= 1) mx = __vmaxu2(mx, __shfl_xor_sync(FULL, mx, o));
+          amax = __uint_as_float(max(mx << 16, mx & 0xffff0000u));
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             v[2 * e] = __uint_as_float(w4[e] << 16);
             v[2 * e + 1] = __uint_as_float(w4[e] & 0xffff0000u);
           }
         }
-        float amax = 0.f, f, inv;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
-#pragma unroll
-        for (int o = LPR / 2; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, o));
         fp4_row_factor(amax, f, inv);
         if (ch == 0) qfac[tile * 128 + rw] = inv * a.qscale;
         uint32_t u[4], lo[4];
@@ -773,21 +783,43 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
         }
       }
     };
-    const int g = row & (G - 1);
     const bool writer = t < C::NS && (t == 0 || wide);  // this warpgroup's rows are the item's
     const size_t part = ((size_t)item * a.Hkv + h) * a.n_split;  // first run of this item and head
     T* out = reinterpret_cast<T*>(a.out);
     if (runs == 1) {
       if (writer && ok && warp_live) {
         const float inv = l > 0.f ? a.v_scale / l : (l == l ? 0.f : l);
-        T* dst = out + ((size_t)(q0 + tb + tile * TT + tok) * a.Hq + h * G + g) * D;
+        // a warp's 32 rows go through shared memory, 16-byte chunks permuted by row, so that a
+        // store writes whole rows and not 16 bytes of each of 32
+        constexpr int CPR = D * (int)sizeof(T) / 16;  // chunks of a row
+        uint4* stage = reinterpret_cast<uint4*>(smem + (C::NS == 1 ? 0u : C::K0) + t * 128u * D * sizeof(T)) +
+                       (warp & 3) * 32 * CPR;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
           columns(c, v);
+          constexpr int CPC = 32 * (int)sizeof(T) / 16;  // chunks of 32 columns
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] *= inv;
-          if (live) store_vec<T, 32>(dst + c * 32, v);
+          for (int i = 0; i < CPC; ++i) {
+            uint4 x;
+            if constexpr (F32) {
+              x = make_uint4(__float_as_uint(v[4 * i] * inv), __float_as_uint(v[4 * i + 1] * inv),
+                             __float_as_uint(v[4 * i + 2] * inv), __float_as_uint(v[4 * i + 3] * inv));
+            } else {
+              x = make_uint4(pack_bf16x2(v[8 * i] * inv, v[8 * i + 1] * inv), pack_bf16x2(v[8 * i + 2] * inv, v[8 * i + 3] * inv),
+                             pack_bf16x2(v[8 * i + 4] * inv, v[8 * i + 5] * inv), pack_bf16x2(v[8 * i + 6] * inv, v[8 * i + 7] * inv));
+            }
+            stage[lane * CPR + ((c * CPC + i) ^ (lane & 7))] = x;
+          }
+        }
+        __syncwarp();
+        const int row0 = (warp & 3) * 32;
+#pragma unroll 4
+        for (int i = lane; i < 32 * CPR; i += 32) {
+          const int rr = i / CPR, ch = i % CPR, rw = row0 + rr, tk = rw >> a.g_log2;
+          if (tk < nq_t[t])
+            reinterpret_cast<uint4*>(out + ((size_t)(q0 + tb + tile * TT + tk) * a.Hq + h * G + (rw & (G - 1))) * D)[ch] =
+                stage[rr * CPR + (ch ^ (rr & 7))];
         }
       }
     } else {
@@ -821,21 +853,30 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
           float M = kNegInf, Ls = 0.f, acc[EPT];
 #pragma unroll
           for (int e = 0; e < EPT; ++e) acc[e] = 0.f;
-          for (int s = 0; s < runs; ++s) {
-            const size_t pr = (part + s) * kF4Rows + i;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + pr * 2));
-            if (ml.x == kNegInf) continue;
-            const float Mn = fmaxf(M, ml.x);
-            const float keep = M == kNegInf ? 0.f : exp2f(M - Mn), wgt = exp2f(ml.x - Mn);
-            Ls = Ls * keep + ml.y * wgt;
-            const float2* src = reinterpret_cast<const float2*>(a.ws_acc + pr * D + lane * EPT);
+          for (int s0 = 0; s0 < runs; s0 += 4) {
+            float2 ml[4], v[4][EPT / 2];
 #pragma unroll
-            for (int e = 0; e < EPT / 2; ++e) {
-              const float2 v = __ldcg(src + e);
-              acc[2 * e] = acc[2 * e] * keep + v.x * wgt;
-              acc[2 * e + 1] = acc[2 * e + 1] * keep + v.y * wgt;
+            for (int u = 0; u < 4; ++u) {
+              const size_t pr = (part + min(s0 + u, runs - 1)) * kF4Rows + i;
+              ml[u] = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + pr * 2));
+              if (s0 + u >= runs) ml[u] = make_float2(kNegInf, 0.f);
+              const float2* src = reinterpret_cast<const float2*>(a.ws_acc + pr * D + lane * EPT);
+#pragma unroll
+              for (int e = 0; e < EPT / 2; ++e) v[u][e] = __ldcg(src + e);
             }
-            M = Mn;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              if (ml[u].x == kNegInf) continue;  // no visible key in this run: its row was not written
+              const float Mn = fmaxf(M, ml[u].x);
+              const float keep = M == kNegInf ? 0.f : exp2f(M - Mn), wgt = exp2f(ml[u].x - Mn);
+              Ls = Ls * keep + ml[u].y * wgt;
+#pragma unroll
+              for (int e = 0; e < EPT / 2; ++e) {
+                acc[2 * e] = acc[2 * e] * keep + v[u][e].x * wgt;
+                acc[2 * e + 1] = acc[2 * e + 1] * keep + v[u][e].y * wgt;
+              }
+              M = Mn;
+            }
           }
           const float inv = Ls > 0.f ? a.v_scale / Ls : (Ls != Ls ? Ls : 0.f);
 #pragma unroll
