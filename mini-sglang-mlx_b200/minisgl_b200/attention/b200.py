@@ -312,22 +312,30 @@ class B200AttnBackend(BaseAttnBackend):
     PACK_PAGE = 16
 
     # ------------------------------------------------------------ prefill metadata built on the device
-    def alloc_extend_metadata(self, batch_size: int, total_q: int, total_pages: int,
-                              tile_q: int | None = None) -> B200PrefillMetadata:
+    @property
+    def device_extend(self) -> bool:
+        """Whether this pool's extend takes tables built on the device (else: host-built key groups)."""
+        P = self.page_size
+        return self.fp4 or P >= self.PACK_PAGE or self._tile_q(P) == self._tile_q(self.PACK_PAGE)
+
+    def alloc_extend_metadata(self, batch_size: int, total_q: int, total_pages: int, tile_q: int | None = None,
+                              cached: np.ndarray | None = None, lens: np.ndarray | None = None) -> B200PrefillMetadata:
         """Prefill metadata of ``batch_size`` requests for ``build_extend_metadata_device`` to fill.
 
         ``total_q`` new tokens and ``total_pages`` pages in all: what the batch needs, or the
         capacity of a batch whose lengths are known on the device only (a captured step). A batch
         that needs less leaves the tails of ``positions``, ``out_loc`` and ``kv_indices`` as they
         were, and empty tiles at the end of ``work``. ``tile_q`` defaults to the tile of this
-        backend's extend kernel.
+        backend's extend kernel. Host copies of ``cached`` and ``lens``, where the caller has
+        them, let a 4-bit pool cut long requests' keys into runs as evenly as
+        ``extend_metadata_from_lens`` does; without them it assumes requests of equal length.
         """
         P = self.page_size
         if tile_q is None:
-            tile_q = self._tile_q(P)
-            if P < self.PACK_PAGE and tile_q != self._tile_q(self.PACK_PAGE):
+            if not self.device_extend:
                 raise ValueError(f"alloc_extend_metadata: page size {P} needs the host-built key groups "
                                  "(extend_metadata_from_lens)")
+            tile_q = self._tile_q(P)
         if batch_size < 1 or total_q < 0 or total_pages < 0 or tile_q < 1:
             raise ValueError(f"alloc_extend_metadata: batch {batch_size}, {total_q} tokens, {total_pages} pages, "
                              f"tile {tile_q}")
@@ -342,8 +350,12 @@ class B200AttnBackend(BaseAttnBackend):
             work=work.view(-1, 4), n_work=n_work, total_q=total_q, page_size=P, positions=pos, out_loc=loc,
             counts=counts, tile_q=tile_q)
         if self.fp4 and n_work:
-            # the lengths are known on the device only: as if every item saw an even share of the pages
-            self._split_extend(meta, np.full(n_work, min(total_pages * P // batch_size, self.page_table.shape[1])))
+            if cached is not None and lens is not None:
+                ends = [np.minimum(np.arange(c + tile_q, n + tile_q, tile_q), n) for c, n in zip(cached, lens)]
+                self._split_extend(meta, np.concatenate(ends))
+            else:
+                even = min(total_pages * P // batch_size, self.page_table.shape[1])
+                self._split_extend(meta, np.full(n_work, even))
         return meta
 
     def build_extend_metadata_device(self, meta: B200PrefillMetadata, page_table: torch.Tensor, rows: torch.Tensor,

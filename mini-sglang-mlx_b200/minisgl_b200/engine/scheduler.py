@@ -55,8 +55,9 @@ class EngineConfig:
     cache_type: str = "radix"
     overlap_scheduling: bool = True
     cuda_graph_max_bs: int = 128  # decode batches up to this size replay CUDA graphs (0: eager)
-    # keep a device copy of the page table; CUDA-graph decode steps then build their
-    # attention metadata on the device, inside the graph (b2a_decode_metadata)
+    # keep a device copy of the page table; CUDA-graph decode steps then build their attention
+    # metadata on the device, inside the graph (b2a_decode_metadata), prefill steps their index
+    # tables in one launch (b2a_extend_metadata)
     device_metadata: bool = True
     # bf16 steps of <= 32 tokens run the layers' projections as b2a_proj launches with the
     # norms, residual adds and SwiGLU fused in (False: cuBLAS + separate kernels throughout)
@@ -212,6 +213,9 @@ class Scheduler(HostScheduler):
 
     def _prepare(self, batch: Batch) -> None:
         reqs = batch.reqs
+        if batch.is_prefill and self.engine.page_table_dev is not None and self.engine.attn_backend.device_extend:
+            self._prepare_prefill_device(batch)
+            return
         positions, out_loc = batch_positions_out_loc(batch, self.engine.page_table)
         rows = np.array([r.table_idx for r in reqs], dtype=np.int32)
         if batch.is_decode and self.graphs is not None and self.graphs.bucket_for(batch.size) is not None:
@@ -240,6 +244,30 @@ class Scheduler(HostScheduler):
         batch.rows = dev[2]
         batch.input_ids = dev[3] if batch.is_prefill else self.table.token_pool[dev[2].long()]
         self.engine.attn_backend.prepare_metadata(batch)
+
+    def _prepare_prefill_device(self, batch: Batch) -> None:
+        """Prefill inputs with the index tables built on the GPU (b2a_extend_metadata).
+
+        The host uploads the tokens, three lengths per request and the page-table entries this
+        step makes valid (a request's whole row so far: its prefix-cache hit was written on the
+        host when it was admitted); positions, slots, CSRs and the work list follow from the
+        device page table, with the values that ``prepare_metadata`` computes on the host.
+        """
+        reqs, be = batch.reqs, self.engine.attn_backend
+        rows = np.array([r.table_idx for r in reqs], dtype=np.int32)
+        cached = np.array([r.cached_len for r in reqs], dtype=np.int32)
+        lens = np.array([r.device_len for r in reqs], dtype=np.int32)
+        ids = np.concatenate([r.input_ids[r.cached_len: r.device_len] for r in reqs]).astype(np.int32)
+        cols = np.concatenate([np.arange(n, dtype=np.int32) for n in lens.tolist()])
+        r_tok = np.repeat(rows, lens)
+        dev = self._stager.upload([rows, cached, lens, ids, r_tok, cols, self.engine.page_table[r_tok, cols]],
+                                  self.engine.device)
+        page_table_scatter(self.engine.page_table_dev, *dev[4:])
+        P = self.cfg.page_size
+        meta = be.alloc_extend_metadata(len(reqs), len(ids), int(((lens + P - 1) // P).sum()), cached=cached, lens=lens)
+        be.build_extend_metadata_device(meta, self.engine.page_table_dev, dev[0], dev[1], dev[2])
+        batch.positions, batch.out_loc, batch.rows, batch.input_ids = meta.positions, meta.out_loc, dev[0], dev[3]
+        batch.attn_metadata = meta
 
     def _forward(self, batch: Batch) -> _Step:
         start = torch.cuda.Event(enable_timing=True)

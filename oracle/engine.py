@@ -45,6 +45,10 @@ class OracleQwen3:
             self.layers.append({k: _np(getattr(L, k)) for k in
                                 ("in_norm", "qkv", "q_norm", "k_norm", "o", "post_norm", "gate_up", "down")})
 
+    def cached(self, k: np.ndarray, v: np.ndarray):
+        """What the KV pool returns for k and v [T, Hkv, D] (a pool of fewer bits overrides this)."""
+        return k, v
+
     def logits_last(self, ids: Sequence[int]) -> np.ndarray:
         """Logits of the last position of the sequence ``ids``."""
         Hq, Hkv, D = self.Hq, self.Hkv, self.D
@@ -61,6 +65,7 @@ class OracleQwen3:
             v = qkv[:, (Hq + Hkv) * D:].reshape(T, Hkv, D)
             q = O.rope(q, pos, self.dims, self.inv_freq)
             k = O.rope(k, pos, self.dims, self.inv_freq)
+            k, v = self.cached(k, v)
             o = np.empty((T, Hq, D))
             for hq in range(Hq):
                 s = (q[:, hq, :] @ k[:, hq // G, :].T) * D ** -0.5
