@@ -420,7 +420,9 @@ int b2a_fp4_decode(const void* q, const void* pool, int64_t num_slots, const int
  * are f32 or bf16 [T, Hq, D], GQA group 1, 2, 4 or 8. `work` comes from
  * b2a_extend_plan or b2a_extend_metadata with the tile size that
  * b2a_fp4_extend_tile_q returns for the same shape; empty tiles at its end are
- * skipped. scale is positive and finite.
+ * skipped. scale is positive and finite. A tile with a request outside [0, B) is
+ * skipped and recorded as device error 35, one that reaches past row T is cut
+ * (error 33).
  * The keys of a work item can be cut into runs of run_keys keys (a multiple of
  * 128), at most n_split (1 to 64) of them, the last one taking what is left:
  * b2a_fp4_extend_runs (host only) proposes both for items whose last token sees
@@ -461,8 +463,8 @@ int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int
  * left as they were (except work). B <= 8192. Lengths outside [0, table_stride],
  * cached lengths outside [0, lens[b]], rows outside the table and entries past a
  * capacity are skipped and recorded as device error 34 (b2a_device_error),
- * negative or unaligned page entries as 32; a work list that does not fit is
- * left empty.
+ * negative or unaligned page entries as 32. A batch that does not fit its
+ * capacities gets an empty work list, so that no attention call reads past them.
  * ------------------------------------------------------------------------ */
 int b2a_extend_metadata(const int32_t* page_table, int64_t table_rows, int64_t table_stride, const int32_t* rows,
                         const int32_t* cached, const int32_t* lens, int B, int page_size, int tile_q,

@@ -1169,15 +1169,15 @@ int b2a_fp4_store_kv(const void* k, int64_t k_row_stride, const void* v, int64_t
   a.row_bytes = b2a::fp4_row_bytes(Hkv, D);
   a.k_scale = k_scale;
   a.v_scale = v_scale;
-  const int64_t blocks = (T * 2 * Hkv * a.nblk + 255) / 256;
+  const int64_t blocks = (T * 2 * Hkv * a.nblk + b2a::kFp4Threads * b2a::kFp4Unroll - 1) / (b2a::kFp4Threads * b2a::kFp4Unroll);
   if (blocks > 0x7fffffff) return fail(B2A_ERR_INVALID, "too many rows");
   const bool vec = aligned(k, 16) && aligned(v, 16) && (k_row_stride * (int64_t)es) % 16 == 0 &&
                    (v_row_stride * (int64_t)es) % 16 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return with_dtype<true>(dtype, [&](auto tag) -> int {
     using Tt = decltype(tag);
-    if (vec) launch_pdl(b2a::fp4_store_kernel<Tt, true>, dim3((unsigned)blocks), dim3(256), 0, st, a);
-    else launch_pdl(b2a::fp4_store_kernel<Tt, false>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    if (vec) launch_pdl(b2a::fp4_store_kernel<Tt, true>, dim3((unsigned)blocks), dim3(b2a::kFp4Threads), 0, st, a);
+    else launch_pdl(b2a::fp4_store_kernel<Tt, false>, dim3((unsigned)blocks), dim3(b2a::kFp4Threads), 0, st, a);
     return check_launch("fp4_store_kernel");
   });
 }
@@ -1204,12 +1204,12 @@ int b2a_fp4_load_kv(const void* pool, int64_t num_slots, const int32_t* slots, i
   a.row_bytes = b2a::fp4_row_bytes(Hkv, D);
   a.k_scale = k_scale;
   a.v_scale = v_scale;
-  const int64_t blocks = (n * 2 * Hkv * a.nblk + 255) / 256;
+  const int64_t blocks = (n * 2 * Hkv * a.nblk + b2a::kFp4Threads * b2a::kFp4Unroll - 1) / (b2a::kFp4Threads * b2a::kFp4Unroll);
   if (blocks > 0x7fffffff) return fail(B2A_ERR_INVALID, "too many rows");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return with_dtype<true>(dtype, [&](auto tag) -> int {
     using Tt = decltype(tag);
-    launch_pdl(b2a::fp4_load_kernel<Tt>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    launch_pdl(b2a::fp4_load_kernel<Tt>, dim3((unsigned)blocks), dim3(b2a::kFp4Threads), 0, st, a);
     return check_launch("fp4_load_kernel");
   });
 }
@@ -1364,6 +1364,8 @@ int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int
   a.num_slots = num_slots;
   a.row_bytes = b2a::fp4_row_bytes(Hkv, D);
   a.page_log2 = plog;
+  a.T = T;
+  a.B = B;
   a.Hq = Hq;
   a.Hkv = Hkv;
   a.G = G;

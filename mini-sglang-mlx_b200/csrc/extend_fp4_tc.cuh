@@ -58,6 +58,7 @@ struct F4Args {
   int64_t num_slots;
   uint32_t row_bytes;
   int page_log2;
+  int T, B;  // rows of q, requests (bounds of the work list)
   int Hq, Hkv, G, g_log2;
   int n_split;   // most runs of an item (grid z)
   int run_keys;  // keys of a run
@@ -211,15 +212,21 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
   const int TT = kTcRows >> a.g_log2;  // tokens per tile
   const int item = a.item0 + blockIdx.y;
   const int4 w = reinterpret_cast<const int4*>(a.work)[item];
-  const int nq = min(w.z, C::WIDE ? 2 * TT : TT);
-  if (nq <= 0) return;  // unused entry behind a device-built work list
-  if (w.z > nq && threadIdx.x == 0) watchdog_set(kWdTileTooLarge);
+  if (w.z <= 0) return;  // unused entry behind a device-built work list
   const int r = w.x, tb = w.y;
+  if (r < 0 || r >= a.B || tb < 0) {
+    if (threadIdx.x == 0) watchdog_set(kWdBadPlan);
+    return;
+  }
+  const int q0 = a.qo_indptr[r];
+  // the tile's tokens, inside the kernel's tile and the rows of q
+  const int nq = min(min(w.z, C::WIDE ? 2 * TT : TT), q0 < 0 ? 0 : a.T - q0 - tb);
+  if (nq < w.z && threadIdx.x == 0) watchdog_set(kWdTileTooLarge);
+  if (nq <= 0) return;
   const bool wide = C::WIDE && nq > TT;
   const int nq_t[2] = {min(nq, TT), wide ? nq - TT : min(nq, TT)};  // tokens of each stream's tile
   const int h = blockIdx.x;
   const int P = 1 << a.page_log2;
-  const int q0 = a.qo_indptr[r];
   const int Lq = a.qo_indptr[r + 1] - q0;
   const int pbeg = a.kv_indptr[r];
   const int npages = a.kv_indptr[r + 1] - pbeg;

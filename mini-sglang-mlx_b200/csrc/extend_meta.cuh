@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
     }
     __syncthreads();
     long long base[3];
-    bool fits = true;
+    bool small = true;
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
       base[c] = inc[c] - s[c];
@@ -149,10 +149,12 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
         if (w == warp) base[c] += all;
         all += wsum[c][w];
       }
-      fits = fits && all <= (c == 2 ? (long long)kEmMaxWork : 0x7fffffffll);
+      small = small && all <= (c == 2 ? (long long)kEmMaxWork : 0x7fffffffll);
     }
-    if (!fits) {  // the same on every thread: the tables stay as they were
+    if (!small) {  // the same on every thread: an empty work list, the other tables as they were
       if (blockIdx.x == 0 && tid == 0) watchdog_set(kWdMetaOverflow);
+      for (int i = blockIdx.x * kEmThreads + tid; i < a.work_capacity; i += gridDim.x * kEmThreads)
+        reinterpret_cast<int4*>(a.work)[i] = make_int4(0, 0, 0, 0);
       return;
     }
     for (int b = b0; b < b1; ++b) {
@@ -167,6 +169,8 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
   }
   __syncthreads();
   const int T = qo[B], NP = kv[B], NT = tl[B];
+  // a batch that does not fit its buffers gets an empty work list: nothing reads past them
+  const bool fits = T <= a.q_capacity && NP <= a.idx_capacity && NT <= a.work_capacity;
   const int gthreads = gridDim.x * kEmThreads;
   const int gid = blockIdx.x * kEmThreads + tid;
 
@@ -182,8 +186,8 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
   }
   if (gid == 0) {
     a.counts[0] = T;
-    a.counts[1] = NT > a.work_capacity ? 0 : NT;
-    if (T > a.q_capacity || NP > a.idx_capacity || NT > a.work_capacity) watchdog_set(kWdMetaOverflow);
+    a.counts[1] = fits ? NT : 0;
+    if (!fits) watchdog_set(kWdMetaOverflow);
   }
 
   // ---- positions and slots of the new tokens
@@ -236,9 +240,9 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
   }
 
   // ---- work list: unused entries are empty tiles, used ones go to their rank
-  for (int i = (NT > a.work_capacity ? 0 : NT) + gid; i < a.work_capacity; i += gthreads)
+  for (int i = (fits ? NT : 0) + gid; i < a.work_capacity; i += gthreads)
     reinterpret_cast<int4*>(a.work)[i] = make_int4(0, 0, 0, 0);
-  if (NT > a.work_capacity) return;  // flagged above, the list stays empty
+  if (!fits) return;
   // key of tile i = tile k of request b: dearer tiles and, among equals, earlier ones are larger
   auto tile_of = [&](int b, int i, int& tb, int& nq) -> unsigned long long {
     tb = (i - tl[b]) * a.tile_q;

@@ -133,80 +133,128 @@ __device__ __forceinline__ void fp4_read16(const T* p, bool vec, float (&x)[16])
   }
 }
 
-// One thread quantises one block of 16 features: 32 or 64 bytes in, 8 + 1 bytes
-// out. Bound by HBM at large T. Neighbouring threads hold neighbouring blocks of
-// a row, so reads and code writes are contiguous over a token's heads.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) fp4_store_kernel(const Fp4KvArgs a) {
-  pdl_wait_then_release();
-  const int64_t per_tok = 2ll * a.Hkv * a.nblk;
-  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
-  if (i >= a.n * per_tok) return;
-  const int64_t t = i / per_tok;
-  const int rem = (int)(i - t * per_tok);
-  const int kind = rem >= a.Hkv * a.nblk;  // 0: k, 1: v
-  const int hb = rem - kind * a.Hkv * a.nblk;
-  const int h = hb / a.nblk, blk = hb - h * a.nblk;
-  const int D = a.nblk * kFp4Block;
-  const int64_t slot = a.slots[t];
-  if (slot < 0 || slot >= a.num_slots) {
-    watchdog_set(kWdBadSlot);
-    return;
-  }
-  const T* src = reinterpret_cast<const T*>(kind ? a.v : a.k) + t * (kind ? a.v_stride : a.k_stride) + hb * kFp4Block;
-  float x[16];
-  fp4_read16<T>(src, VEC, x);
-  const float inv_g = 1.f / (kind ? a.v_scale : a.k_scale);  // exact: a power of two
-  float amax = 0.f;
+// Threads take blocks of 16 features, neighbours neighbouring blocks, so reads and writes are
+// contiguous over a token's heads. HBM bounds both kernels at large n: a thread takes kFp4Unroll
+// blocks kFp4Threads apart, so that many independent slot -> row reads are in flight, and one
+// 64-bit division per CTA finds the first token (a block per thread: 76.7 us for store and load
+// of 16,391 fp32 tokens of 8 x 128 and 148.6 us for the load of 120,001 bf16 ones).
+constexpr int kFp4Threads = 256;
+constexpr int kFp4Unroll = 4;
+
+struct Fp4Where {
+  int64_t t;        // token row of the call
+  int64_t slot;     // pool slot, -1 outside the pool
+  int kind, h, blk; // 0 k / 1 v, kv head, block of the head row
+  bool have;
+};
+
+// The blocks of this thread; `slots` reads go out together.
+__device__ __forceinline__ void fp4_where(const Fp4KvArgs& a, Fp4Where (&w)[kFp4Unroll]) {
+  const uint32_t half = (uint32_t)(a.Hkv * a.nblk), per_tok = 2u * half;
+  const int64_t i0 = (int64_t)blockIdx.x * (kFp4Threads * kFp4Unroll);
+  const int64_t t0 = i0 / per_tok;
+  const uint32_t r0 = (uint32_t)(i0 - t0 * per_tok) + threadIdx.x;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    x[j] = (x[j] != x[j]) ? 0.f : x[j] * inv_g;
-    amax = fmaxf(amax, fabsf(x[j]));
+  for (int u = 0; u < kFp4Unroll; ++u) {
+    const uint32_t r = r0 + u * kFp4Threads, dt = r / per_tok;
+    uint32_t e = r - dt * per_tok;
+    w[u].t = t0 + dt;
+    w[u].kind = e >= half;
+    e -= w[u].kind ? half : 0u;
+    w[u].h = (int)(e / (uint32_t)a.nblk);
+    w[u].blk = (int)(e - (uint32_t)w[u].h * a.nblk);
+    w[u].have = w[u].t < a.n;
+    w[u].slot = w[u].have ? a.slots[w[u].t] : 0;
   }
-  const uint32_t sb = f_to_e4m3(fminf(__fdiv_rn(amax, 6.f), 448.f));
-  const uint32_t sh = fp4_scale2_to_h2(sb);
-  const float s = __half2float(__ushort_as_half((unsigned short)(sh & 0xffffu)));
-  uint32_t w[2] = {0u, 0u};
-  if (s > 0.f) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      w[j >> 2] |= f2_to_e2m1(__fdiv_rn(x[2 * j], s), __fdiv_rn(x[2 * j + 1], s)) << (8 * (j & 3));
+  for (int u = 0; u < kFp4Unroll; ++u) {
+    if (w[u].slot < 0 || w[u].slot >= a.num_slots) {
+      watchdog_set(kWdBadSlot);
+      w[u].slot = -1;
+    }
   }
-  uint8_t* row = a.pool + (size_t)slot * a.row_bytes;
-  *reinterpret_cast<uint2*>(row + fp4_code_off(h, D) + kind * (D / 2) + blk * 8) = make_uint2(w[0], w[1]);
-  row[fp4_scale_off(h, a.Hkv, D) + kind * a.nblk + blk] = (uint8_t)sb;
 }
 
-// One thread expands one block of 16: 8 + 1 bytes in, 32 or 64 bytes out.
-template <typename T>
-__global__ void __launch_bounds__(256) fp4_load_kernel(const Fp4KvArgs a) {
+// x / s to nearest for |x| <= 2^13 and an e4m3 s > 0 with y = 1 / s to nearest: Markstein's
+// correction of x * y by its remainder ("Computation of elementary functions on the IBM RISC
+// System/6000 processor", 1990), three operations instead of a division per element. The
+// remainder is exact unless x is so small that the code is zero either way.
+__device__ __forceinline__ float fp4_quotient(float x, float s, float y) {
+  const float q = x * y;
+  return fmaf(fmaf(-q, s, x), y, q);
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kFp4Threads) fp4_store_kernel(const Fp4KvArgs a) {
   pdl_wait_then_release();
-  const int64_t per_tok = 2ll * a.Hkv * a.nblk;
-  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
-  if (i >= a.n * per_tok) return;
-  const int64_t t = i / per_tok;
-  const int rem = (int)(i - t * per_tok);
-  const int kind = rem >= a.Hkv * a.nblk;
-  const int hb = rem - kind * a.Hkv * a.nblk;
-  const int h = hb / a.nblk, blk = hb - h * a.nblk;
+  Fp4Where w[kFp4Unroll];
+  fp4_where(a, w);
   const int D = a.nblk * kFp4Block;
-  const int64_t slot = a.slots[t];
-  uint2 c = make_uint2(0u, 0u);  // a slot outside the pool reads as zeros
-  uint32_t sb = 0;
-  if (slot < 0 || slot >= a.num_slots) {
-    watchdog_set(kWdBadSlot);
-  } else {
-    const uint8_t* row = a.pool + (size_t)slot * a.row_bytes;
-    c = *reinterpret_cast<const uint2*>(row + fp4_code_off(h, D) + kind * (D / 2) + blk * 8);
-    sb = row[fp4_scale_off(h, a.Hkv, D) + kind * a.nblk + blk];
-  }
-  const float g = kind ? a.v_scale : a.k_scale;
-  float x[16];
-  fp4_expand16(c, sb, x);
 #pragma unroll
-  for (int j = 0; j < 16; ++j) x[j] *= g;
-  T* dst = reinterpret_cast<T*>(kind ? a.v_out : a.k_out) + (t * a.Hkv * a.nblk + hb) * kFp4Block;
-  store_vec<T, 16>(dst, x);
+  for (int u = 0; u < kFp4Unroll; ++u) {
+    if (!w[u].have || w[u].slot < 0) continue;
+    const T* src = reinterpret_cast<const T*>(w[u].kind ? a.v : a.k) + w[u].t * (w[u].kind ? a.v_stride : a.k_stride) +
+                   (w[u].h * a.nblk + w[u].blk) * kFp4Block;
+    float x[16];
+    fp4_read16<T>(src, VEC, x);
+    const float inv_g = 1.f / (w[u].kind ? a.v_scale : a.k_scale);  // exact: a power of two
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      x[j] = (x[j] != x[j]) ? 0.f : x[j] * inv_g;
+      amax = fmaxf(amax, fabsf(x[j]));
+    }
+    const uint32_t sb = f_to_e4m3(fminf(__fdiv_rn(amax, 6.f), 448.f));
+    const uint32_t sh = fp4_scale2_to_h2(sb);
+    const float s = __half2float(__ushort_as_half((unsigned short)(sh & 0xffffu)));
+    uint32_t c[2] = {0u, 0u};
+    if (s > 0.f) {
+      const float y = __fdiv_rn(1.f, s);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        // 8192 / 448 is past the largest border: clipping changes no code and keeps infinities out
+        x[j] = fp4_quotient(fminf(fmaxf(x[j], -8192.f), 8192.f), s, y);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j >> 2] |= f2_to_e2m1(x[2 * j], x[2 * j + 1]) << (8 * (j & 3));
+    }
+    uint8_t* row = a.pool + (size_t)w[u].slot * a.row_bytes;
+    *reinterpret_cast<uint2*>(row + fp4_code_off(w[u].h, D) + w[u].kind * (D / 2) + w[u].blk * 8) = make_uint2(c[0], c[1]);
+    row[fp4_scale_off(w[u].h, a.Hkv, D) + w[u].kind * a.nblk + w[u].blk] = (uint8_t)sb;
+  }
+}
+
+// 8 + 1 bytes of a block in, 32 or 64 out.
+template <typename T>
+__global__ void __launch_bounds__(kFp4Threads) fp4_load_kernel(const Fp4KvArgs a) {
+  pdl_wait_then_release();
+  Fp4Where w[kFp4Unroll];
+  fp4_where(a, w);
+  const int D = a.nblk * kFp4Block;
+  uint2 c[kFp4Unroll];
+  uint32_t sb[kFp4Unroll];
+#pragma unroll
+  for (int u = 0; u < kFp4Unroll; ++u) {
+    c[u] = make_uint2(0u, 0u);  // a slot outside the pool reads as zeros
+    sb[u] = 0;
+    if (w[u].slot >= 0) {
+      const uint8_t* row = a.pool + (size_t)w[u].slot * a.row_bytes;
+      c[u] = __ldg(reinterpret_cast<const uint2*>(row + fp4_code_off(w[u].h, D) + w[u].kind * (D / 2) + w[u].blk * 8));
+      sb[u] = __ldg(row + fp4_scale_off(w[u].h, a.Hkv, D) + w[u].kind * a.nblk + w[u].blk);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kFp4Unroll; ++u) {
+    if (!w[u].have) continue;
+    const float g = w[u].kind ? a.v_scale : a.k_scale;
+    float x[16];
+    fp4_expand16(c[u], sb[u], x);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] *= g;
+    T* dst = reinterpret_cast<T*>(w[u].kind ? a.v_out : a.k_out) +
+             (w[u].t * a.Hkv * a.nblk + w[u].h * a.nblk + w[u].blk) * kFp4Block;
+    store_vec<T, 16>(dst, x);
+  }
 }
 
 }  // namespace b2a

@@ -166,6 +166,7 @@ def test_bad_lengths_are_flagged():
         meta = be.alloc_extend_metadata(B, t, p, tile_q=64)
         be.build_extend_metadata_device(meta, _i32(table), _i32(rows), _i32(lens - ext), _i32(lens))
         assert _device_error() == 34
+        assert (meta.work == 0).all() and int(meta.counts[1]) == 0  # nothing is attended
 
 
 def test_refusals():

@@ -340,6 +340,24 @@ def test_a_bad_page_is_reported():
     assert _device_error() == 32
 
 
+def test_bad_tiles_are_skipped():
+    """A work list with a request out of range, or with more tokens than q has rows, stays in bounds."""
+    from minisgl_b200 import B200AttnBackend
+
+    p = Pool([64, 32], 8, 128, "bfloat16", 16, seed=9)
+    be = B200AttnBackend(HeadConfig(16, 8, 128), p.cache, p.pb.page_table, 16)
+    q = to_dev(rand(p.rng, (2, 16, 128), "bfloat16"), "bfloat16")
+    want = be._forward_prefill(q, None, None, 0, be.extend_metadata_from_lens(p.pb.rows, p.pb.lens, np.array([1, 1])))
+    for i, bad, code in ((0, 7, 35), (0, -1, 35), (2, 9, 33)):
+        meta = be.extend_metadata_from_lens(p.pb.rows, p.pb.lens, np.array([1, 1]))
+        last = int((meta.work[:, 0] == 1).nonzero()[0])  # request 1's tile
+        meta.work[last, i] = bad
+        assert _device_error() == 0
+        out = be._forward_prefill(q, None, None, 0, meta)
+        assert _device_error() == code
+        assert bool((out[0] == want[0]).all())
+
+
 def test_python_refusals():
     import torch
 
