@@ -1204,7 +1204,8 @@ int b2a_fp4_load_kv(const void* pool, int64_t num_slots, const int32_t* slots, i
   a.row_bytes = b2a::fp4_row_bytes(Hkv, D);
   a.k_scale = k_scale;
   a.v_scale = v_scale;
-  const int64_t blocks = (n * 2 * Hkv * a.nblk + b2a::kFp4Threads * b2a::kFp4Unroll - 1) / (b2a::kFp4Threads * b2a::kFp4Unroll);
+  const int64_t units = n * 2 * Hkv * a.nblk;
+  const int64_t blocks = (units + b2a::kFp4Threads * b2a::kFp4Unroll - 1) / (b2a::kFp4Threads * b2a::kFp4Unroll);
   if (blocks > 0x7fffffff) return fail(B2A_ERR_INVALID, "too many rows");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return with_dtype<true>(dtype, [&](auto tag) -> int {

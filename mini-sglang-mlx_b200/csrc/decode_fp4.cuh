@@ -21,6 +21,12 @@
 // before they are expanded, so an operand register holds one feature of two
 // tokens without any shuffle.
 //
+// What is left. 72 requests of 1k to 32k tokens (32 / 8 heads x 128, 1.35 GB) take 268 us, 5.0
+// TB/s; the same stream without the arithmetic takes 220 us, the arithmetic on resident rows 240.
+// The core (64 conversions, 64 packed multiplies, 16 MMAs a unit) runs at 86 clocks a unit of an
+// SM's 99 at HBM rate: m16n8k16 MMAs and the packed multiplies share a pipe (2.07 and 0.51 clocks
+// each, measured to add up), which binds it more than instruction issue does.
+//
 // q enters as fp16 with each head row scaled by a power of two so that its
 // largest element lies in [2^14, 2^15): bf16 has 8 significant bits, so only
 // elements 2^28 times smaller than the largest lose any. The factor goes back
@@ -38,7 +44,7 @@
 namespace b2a {
 
 // units of 16 tokens a warp takes at a time
-// (measured at 8 kv heads x 128, 72 requests of 16k tokens: 332, 330, 282 us for 1, 2, 4
+// (measured at 8 kv heads x 128, 72 requests of 1k to 32k tokens: 332, 330, 282 us for 1, 2, 4
 // units; 16 warps of 2 units, which need a combine per segment: 303 us). Four units of
 // head_dim 256 would leave room for one stage, and 16 warps have registers for one unit.
 __host__ __device__ constexpr int fp4_units_of(int NCW, int D) { return NCW == 16 ? 1 : D == 256 ? 2 : 4; }

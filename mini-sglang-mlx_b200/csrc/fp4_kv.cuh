@@ -89,24 +89,6 @@ __device__ __forceinline__ uint32_t f2_to_e2m1(float lo, float hi) {
   return r;
 }
 
-// The sixteen values of a block (before the pool's own factor), exact.
-__device__ __forceinline__ void fp4_expand16(uint2 codes, uint32_t scale_byte, float (&x)[16]) {
-  const uint32_t sh = fp4_scale2_to_h2(scale_byte | (scale_byte << 8));
-  uint32_t r0[4], r1[4];
-  fp4_word_to_h2(codes.x, r0);
-  fp4_word_to_h2(codes.y, r1);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = h2_mul(r0[j], sh), hi = h2_mul(r1[j], sh);
-    const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-    const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    x[2 * j] = f0.x;
-    x[2 * j + 1] = f0.y;
-    x[8 + 2 * j] = f1.x;
-    x[9 + 2 * j] = f1.y;
-  }
-}
-
 struct Fp4KvArgs {
   const void* k;  // store: new rows
   const void* v;
@@ -136,21 +118,22 @@ __device__ __forceinline__ void fp4_read16(const T* p, bool vec, float (&x)[16])
 // Threads take blocks of 16 features, neighbours neighbouring blocks, so reads and writes are
 // contiguous over a token's heads. HBM bounds both kernels at large n: a thread takes kFp4Unroll
 // blocks kFp4Threads apart, so that many independent slot -> row reads are in flight, and one
-// 64-bit division per CTA finds the first token (a block per thread: 76.7 us for store and load
-// of 16,391 fp32 tokens of 8 x 128 and 148.6 us for the load of 120,001 bf16 ones).
+// 64-bit division per thread finds the first token. Store and load of 16,391 fp32 tokens of
+// 8 x 128 take 71 us (a block and a division per thread: 77), the load of 120,001 bf16 ones
+// 126 us, 5.0 TB/s (149).
 constexpr int kFp4Threads = 256;
 constexpr int kFp4Unroll = 4;
 
 struct Fp4Where {
   int64_t t;        // token row of the call
   int64_t slot;     // pool slot, -1 outside the pool
-  int kind, h, blk; // 0 k / 1 v, kv head, block of the head row
+  int kind, h, blk; // 0 k / 1 v, kv head, unit of the head row
   bool have;
 };
 
-// The blocks of this thread; `slots` reads go out together.
-__device__ __forceinline__ void fp4_where(const Fp4KvArgs& a, Fp4Where (&w)[kFp4Unroll]) {
-  const uint32_t half = (uint32_t)(a.Hkv * a.nblk), per_tok = 2u * half;
+// The units of this thread, npr of them in a head row; `slots` reads go out together.
+__device__ __forceinline__ void fp4_where(const Fp4KvArgs& a, int npr, Fp4Where (&w)[kFp4Unroll]) {
+  const uint32_t half = (uint32_t)(a.Hkv * npr), per_tok = 2u * half;
   const int64_t i0 = (int64_t)blockIdx.x * (kFp4Threads * kFp4Unroll);
   const int64_t t0 = i0 / per_tok;
   const uint32_t r0 = (uint32_t)(i0 - t0 * per_tok) + threadIdx.x;
@@ -161,8 +144,8 @@ __device__ __forceinline__ void fp4_where(const Fp4KvArgs& a, Fp4Where (&w)[kFp4
     w[u].t = t0 + dt;
     w[u].kind = e >= half;
     e -= w[u].kind ? half : 0u;
-    w[u].h = (int)(e / (uint32_t)a.nblk);
-    w[u].blk = (int)(e - (uint32_t)w[u].h * a.nblk);
+    w[u].h = (int)(e / (uint32_t)npr);
+    w[u].blk = (int)(e - (uint32_t)w[u].h * npr);
     w[u].have = w[u].t < a.n;
     w[u].slot = w[u].have ? a.slots[w[u].t] : 0;
   }
@@ -188,7 +171,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kFp4Threads) fp4_store_kernel(const Fp4KvArgs a) {
   pdl_wait_then_release();
   Fp4Where w[kFp4Unroll];
-  fp4_where(a, w);
+  fp4_where(a, a.nblk, w);
   const int D = a.nblk * kFp4Block;
 #pragma unroll
   for (int u = 0; u < kFp4Unroll; ++u) {
@@ -224,13 +207,16 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_store_kernel(const Fp4KvArgs 
   }
 }
 
-// 8 + 1 bytes of a block in, 32 or 64 out.
+// 8 + 1 bytes of a block in, 32 or 64 out. Neighbouring lanes hold neighbouring blocks and
+// exchange 16-byte chunks, so that every store of a pair fills whole 32-byte sectors.
 template <typename T>
 __global__ void __launch_bounds__(kFp4Threads) fp4_load_kernel(const Fp4KvArgs a) {
   pdl_wait_then_release();
-  Fp4Where w[kFp4Unroll];
-  fp4_where(a, w);
+  constexpr int NC = (int)sizeof(T);      // 16-byte chunks of a block
   const int D = a.nblk * kFp4Block;
+  const bool odd = threadIdx.x & 1;
+  Fp4Where w[kFp4Unroll];
+  fp4_where(a, a.nblk, w);
   uint2 c[kFp4Unroll];
   uint32_t sb[kFp4Unroll];
 #pragma unroll
@@ -239,21 +225,54 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_load_kernel(const Fp4KvArgs a
     sb[u] = 0;
     if (w[u].slot >= 0) {
       const uint8_t* row = a.pool + (size_t)w[u].slot * a.row_bytes;
-      c[u] = __ldg(reinterpret_cast<const uint2*>(row + fp4_code_off(w[u].h, D) + w[u].kind * (D / 2) + w[u].blk * 8));
-      sb[u] = __ldg(row + fp4_scale_off(w[u].h, a.Hkv, D) + w[u].kind * a.nblk + w[u].blk);
+      c[u] = *reinterpret_cast<const uint2*>(row + fp4_code_off(w[u].h, D) + w[u].kind * (D / 2) + w[u].blk * 8);
+      sb[u] = row[fp4_scale_off(w[u].h, a.Hkv, D) + w[u].kind * a.nblk + w[u].blk];
     }
   }
 #pragma unroll
   for (int u = 0; u < kFp4Unroll; ++u) {
-    if (!w[u].have) continue;
     const float g = w[u].kind ? a.v_scale : a.k_scale;
-    float x[16];
-    fp4_expand16(c[u], sb[u], x);
+    const uint32_t sh = fp4_scale2_to_h2(sb[u] | (sb[u] << 8));
+    uint4 x[NC];
+    {
+      uint32_t r[8], lo[4], hi[4];
+      fp4_word_to_h2(c[u].x, lo);
+      fp4_word_to_h2(c[u].y, hi);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] *= g;
-    T* dst = reinterpret_cast<T*>(w[u].kind ? a.v_out : a.k_out) +
-             (w[u].t * a.Hkv * a.nblk + w[u].h * a.nblk + w[u].blk) * kFp4Block;
-    store_vec<T, 16>(dst, x);
+      for (int j = 0; j < 4; ++j) {
+        r[j] = h2_mul(lo[j], sh);
+        r[4 + j] = h2_mul(hi[j], sh);
+      }
+      constexpr int PC = 8 / (int)sizeof(T);  // pairs of a chunk
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        float f[2 * PC];
+#pragma unroll
+        for (int j = 0; j < PC; ++j) {
+          const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&r[k * PC + j]));
+          f[2 * j] = p.x * g;
+          f[2 * j + 1] = p.y * g;
+        }
+        store_vec<T, 2 * PC>(reinterpret_cast<T*>(&x[k]), f);
+      }
+    }
+    // a pair's blocks lie next to each other in one token row (an even number of blocks a head)
+    T* pair = reinterpret_cast<T*>(w[u].kind ? a.v_out : a.k_out) +
+              ((w[u].t * a.Hkv + w[u].h) * (int64_t)a.nblk + (w[u].blk & ~1)) * kFp4Block;
+    uint4* dst = reinterpret_cast<uint4*>(pair);
+#pragma unroll
+    for (int k = 0; k < NC; k += 2) {
+      const uint4 give = odd ? x[k] : x[k + 1];
+      uint4 got;
+      got.x = __shfl_xor_sync(0xffffffffu, give.x, 1);
+      got.y = __shfl_xor_sync(0xffffffffu, give.y, 1);
+      got.z = __shfl_xor_sync(0xffffffffu, give.z, 1);
+      got.w = __shfl_xor_sync(0xffffffffu, give.w, 1);
+      if (w[u].have) {
+        dst[k + odd] = odd ? got : x[k];
+        dst[NC + k + odd] = odd ? x[k + 1] : got;
+      }
+    }
   }
 }
 
