@@ -112,8 +112,6 @@ def test_pool_scales(gk, gv):
 @pytest.mark.parametrize("off", [0, 1, 3])
 def test_store_of_strided_and_unaligned_rows(off):
     """k, v as views of a fused projection, at any element offset."""
-    import torch
-
     T, Hq, Hkv, D = 21, 4, 2, 64
     rng = np.random.default_rng(off)
     w = (Hq + 2 * Hkv) * D + off
@@ -125,7 +123,6 @@ def test_store_of_strided_and_unaligned_rows(off):
     c.store_kv(k, v, _i32(loc), 0)
     np.testing.assert_array_equal(c.rows(0).cpu().numpy()[loc],
                                   F.pack_rows(k.float().cpu().numpy(), v.float().cpu().numpy()))
-    assert torch.cuda.current_stream().query() in (True, False)
 
 
 def test_slots_outside_the_pool_are_skipped():
@@ -274,7 +271,7 @@ def test_decode_magnitudes(dtype):
         _check(out, refs, dtype, D, max(lens))
 
 
-EXTEND_SHAPES = [(16, 8, 128), (8, 8, 128), (32, 8, 128), (8, 1, 128), (6, 3, 128), (4, 2, 64), (8, 8, 64),
+EXTEND_SHAPES = [(16, 8, 128), (8, 8, 128), (32, 8, 128), (8, 1, 128), (4, 2, 64), (8, 8, 64),
                  (16, 2, 64), (4, 2, 256), (16, 2, 256)]
 
 
@@ -284,13 +281,11 @@ def _extend_case(Hq, Hkv, D, dtype, P, lens, ext, seed, **kw):
     p = Pool(lens, Hkv, D, dtype, P, seed=seed, **kw)
     lens, ext = np.asarray(lens), np.asarray(ext)
     q = rand(p.rng, (int(ext.sum()), Hq, D), dtype)
-    be = object.__new__(B200AttnBackend)
-    B200AttnBackend.__init__(be, HeadConfig(Hq, Hkv, D), p.cache, p.pb.page_table, P) if Hkv in (1, 2, 4, 8, 16) else None
-    return p, lens, ext, q, be
+    return p, lens, ext, q, B200AttnBackend(HeadConfig(Hq, Hkv, D), p.cache, p.pb.page_table, P)
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
-@pytest.mark.parametrize("Hq,Hkv,D", [s for s in EXTEND_SHAPES if s[1] in (1, 2, 4, 8, 16)])
+@pytest.mark.parametrize("Hq,Hkv,D", EXTEND_SHAPES)
 def test_extend_shapes(Hq, Hkv, D, dtype):
     lens, ext = [1, 40, 130, 17, 300, 129], [1, 40, 2, 16, 77, 1]
     p, lens, ext, q, be = _extend_case(Hq, Hkv, D, dtype, 16, lens, ext, seed=Hq + D)
@@ -321,6 +316,36 @@ def test_extend_page_sizes(P, dtype):
         o += n
     _check(out, refs, dtype, D, int(lens.max()))
     assert _device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 1, 128), (4, 1, 64), (2, 2, 256), (8, 1, 128)])
+def test_extend_long_prompts_in_runs(Hq, Hkv, D, dtype):
+    """One long prompt: tiles whose keys are cut into runs, the first tile of a pair needing fewer
+    blocks than the second, and a last run shorter than the others."""
+    for L, n, run_keys in ((1500, 250, None), (1500, 250, 128), (900, 900, 640), (2049, 65, 256)):
+        p, lens, ext, q, be = _extend_case(Hq, Hkv, D, dtype, 16, [L], [n], seed=L + D, spike=4.0)
+        meta = be.extend_metadata_from_lens(p.pb.rows, lens, ext)
+        if run_keys is None:
+            assert meta.n_split > 1
+        else:
+            _force_runs(be, meta, run_keys, -(-L // run_keys))
+        out = be._forward_prefill(to_dev(q, dtype), None, None, 0, meta)
+        again = be._forward_prefill(to_dev(q, dtype), None, None, 0, meta)
+        assert bool((out == again).all()), "extend is not repeatable"
+        _check(out, [F.attend(q.astype(np.float64), *p.of(0), be.scale, L - n)], dtype, D, L)
+    assert _device_error() == 0
+
+
+def _force_runs(be, meta, run_keys, n_split):
+    """Another cut of the same work items, with a workspace for it."""
+    import torch
+
+    from minisgl_b200 import _native as nat
+
+    meta.run_keys, meta.n_split = run_keys, n_split
+    n = int(nat.LIB.b2a_fp4_extend_workspace_bytes(meta.n_work, n_split, be.Hkv, be.D))
+    meta.workspace = torch.zeros(n, dtype=torch.uint8, device="cuda")
 
 
 def test_a_bad_page_is_reported():
