@@ -21,8 +21,8 @@
 // before they are expanded, so an operand register holds one feature of two
 // tokens without any shuffle.
 //
-// What is left. 72 requests of 1k to 32k tokens (32 / 8 heads x 128, 1.35 GB) take 268 us, 5.0
-// TB/s; the same stream without the arithmetic takes 220 us, the arithmetic on resident rows 240.
+// What is left. 72 requests of 1k to 32k tokens (32 / 8 heads x 128, 1.35 GB) take 268 to 288
+// us in different runs, 4.7 to 5.0 TB/s; the same stream without the arithmetic takes 220 us, the arithmetic on resident rows 240.
 // The core (64 conversions, 64 packed multiplies, 16 MMAs a unit) runs at 86 clocks a unit of an
 // SM's 99 at HBM rate: m16n8k16 MMAs and the packed multiplies share a pipe (2.07 and 0.51 clocks
 // each, measured to add up), which binds it more than instruction issue does.
