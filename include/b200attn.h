@@ -68,7 +68,10 @@ int b2a_device_error(void* stream, int* code_out);
  * KV-pool store.
  * Replaces MHAKVCache.store_kv (python/minisgl_mlx/kvcache/pool.py:47-50):
  *   k_pool[out_loc[t]] = k[t];  v_pool[out_loc[t]] = v[t]   for t < T.
- * Byte-exact copy. out_loc entries must be unique and < num_slots.
+ * Byte-exact copy. out_loc entries must be unique and < num_slots, or -1: that
+ * row has no slot and is skipped (padding of a captured step). Any other entry
+ * outside the pool is skipped too and recorded as device error 32. The same
+ * holds for every store below.
  * ------------------------------------------------------------------------ */
 int b2a_store_kv(const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride,
                  const int32_t* out_loc, void* k_pool, void* v_pool, int64_t num_slots, int T,
@@ -390,8 +393,9 @@ int b2a_proj(const void* x, int64_t x_row_stride, int M, int K, const void* w, i
  * slots out_loc, which must be unique. dtype f32, bf16 or f16; rows of any
  * alignment. b2a_fp4_load_kv expands the rows of n slots into contiguous
  * [n, Hkv, D] k_out and v_out, exactly for f32 and bf16 (f16 holds every value
- * while k_scale and v_scale are 1). A slot outside the pool is recorded as device
- * error 32; the store skips it, the load returns zeros for it.
+ * while k_scale and v_scale are 1). The store skips rows of slot -1. Any other
+ * slot outside the pool, and -1 for the load, is recorded as device error 32;
+ * the store skips it, the load returns zeros for it.
  * ------------------------------------------------------------------------ */
 size_t b2a_fp4_row_bytes(int Hkv, int D);
 int b2a_fp4_store_kv(const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, const int32_t* out_loc,
@@ -460,11 +464,15 @@ int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int
  *                   aligned; min(B, T) + T / tile_q entries are always enough
  *   counts        : out int32 [2] = {new tokens, tiles}
  * Identical values to the host builders. Entries past what the batch needs are
- * left as they were (except work). B <= 8192. Lengths outside [0, table_stride],
- * cached lengths outside [0, lens[b]], rows outside the table and entries past a
- * capacity are skipped and recorded as device error 34 (b2a_device_error),
- * negative or unaligned page entries as 32. A batch that does not fit its
- * capacities gets an empty work list, so that no attention call reads past them.
+ * left as they were, except work and out_loc: every entry of out_loc behind the
+ * last token is -1, so that a store of all q_capacity rows (a captured step)
+ * writes the batch's own slots only. B <= 8192. Lengths outside
+ * [0, table_stride], cached lengths outside [0, lens[b]], rows outside the table
+ * (their slots and pages become -1) and entries past a capacity are recorded as
+ * device error 34 (b2a_device_error), negative slots and negative or unaligned
+ * page entries as 32. A batch that does not fit its capacities gets an empty work
+ * list and an out_loc of -1, so that no attention call reads past them and no
+ * store follows.
  * ------------------------------------------------------------------------ */
 int b2a_extend_metadata(const int32_t* page_table, int64_t table_rows, int64_t table_stride, const int32_t* rows,
                         const int32_t* cached, const int32_t* lens, int B, int page_size, int tile_q,

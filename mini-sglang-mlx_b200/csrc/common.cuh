@@ -31,6 +31,10 @@ enum WatchdogCode : int {
   kWdBadPlan = 35,       // decode plan: a request id or partial slot outside its bounds: segment skipped
 };
 
+// A pool slot of -1: this row has none (padding of a captured step), the stores skip it. Any
+// other slot outside the pool is an error (kWdBadSlot).
+constexpr int kNoSlot = -1;
+
 __device__ __forceinline__ void watchdog_set(int code) { atomicCAS(&g_watchdog, 0, code); }
 
 // Programmatic dependent launch: kernels launched with the programmatic-stream-

@@ -6,7 +6,9 @@
 // tokens, of which the first cached[b] are in the pool already, E = L - cached[b]:
 //   qo_indptr, kv_indptr   exclusive sums of E and of ceil(L / P)
 //   positions[qo_b + i]    cached[b] + i              (i < E)
-//   out_loc[qo_b + i]      page_table[rows[b], cached[b] + i]
+//   out_loc[qo_b + i]      page_table[rows[b], cached[b] + i]; -1 (no slot: a store skips the row)
+//                          behind the last token, for a row outside the table, and everywhere
+//                          when the batch does not fit its buffers
 //   kv_indices[kv_b + p]   page_table[rows[b], p P] / P
 //   work                   {b, first token, tokens, 0} per tile of tile_q new tokens, by
 //                          falling cost tokens * (keys its last token sees), equal costs
@@ -155,6 +157,8 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
       if (blockIdx.x == 0 && tid == 0) watchdog_set(kWdMetaOverflow);
       for (int i = blockIdx.x * kEmThreads + tid; i < a.work_capacity; i += gridDim.x * kEmThreads)
         reinterpret_cast<int4*>(a.work)[i] = make_int4(0, 0, 0, 0);
+      for (int64_t i = (int64_t)blockIdx.x * kEmThreads + tid; i < a.q_capacity; i += (int64_t)gridDim.x * kEmThreads)
+        a.out_loc[i] = kNoSlot;
       return;
     }
     for (int b = b0; b < b1; ++b) {
@@ -190,30 +194,35 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
     if (!fits) watchdog_set(kWdMetaOverflow);
   }
 
-  // ---- positions and slots of the new tokens
+  // ---- positions and slots of the new tokens. Every entry of out_loc is written: a captured step
+  // stores as many rows as the buffer has, and a slot left from another batch may be in use
   const int Tc = (int)min((int64_t)T, a.q_capacity);
   for (int64_t i0 = gid; i0 < Tc; i0 += 4ll * gthreads) {
     int pos[4], loc[4];
-    bool have[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int64_t i = i0 + (int64_t)u * gthreads;
-      have[u] = i < Tc;
-      pos[u] = loc[u] = 0;
-      if (have[u]) {
+      pos[u] = 0;
+      loc[u] = kNoSlot;
+      if (i < Tc) {
         const int b = em_find(qo, B, (int)i);
         pos[u] = cached[b] + (int)i - qo[b];
-        have[u] = rows[b] >= 0;
-        if (have[u]) loc[u] = __ldg(a.page_table + (int64_t)rows[b] * a.stride + pos[u]);
+        if (fits && rows[b] >= 0) {
+          loc[u] = __ldg(a.page_table + (int64_t)rows[b] * a.stride + pos[u]);
+          if (loc[u] < 0) watchdog_set(kWdBadSlot);
+        }
       }
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int64_t i = i0 + (int64_t)u * gthreads;
-      if (i < Tc) a.positions[i] = pos[u];
-      if (have[u]) a.out_loc[i] = loc[u];
+      if (i < Tc) {
+        a.positions[i] = pos[u];
+        a.out_loc[i] = loc[u];
+      }
     }
   }
+  for (int64_t i = (int64_t)Tc + gid; i < a.q_capacity; i += gthreads) a.out_loc[i] = kNoSlot;
 
   // ---- page ids of every request's tokens
   const int NPc = (int)min((int64_t)NP, a.idx_capacity);
@@ -223,9 +232,9 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int64_t i = i0 + (int64_t)u * gthreads;
-      have[u] = i < NPc;
-      e[u] = 0;
-      if (have[u]) {
+      e[u] = -1;  // a row outside the table: no page, attention reads zeros
+      have[u] = false;
+      if (i < NPc) {
         const int b = em_find(kv, B, (int)i);
         have[u] = rows[b] >= 0;
         if (have[u]) e[u] = __ldg(a.page_table + (int64_t)rows[b] * a.stride + ((int64_t)((int)i - kv[b]) << a.page_log2));
@@ -233,9 +242,9 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if (!have[u]) continue;
-      if (e[u] < 0 || (e[u] & (P - 1))) watchdog_set(kWdBadSlot);
-      a.kv_indices[i0 + (int64_t)u * gthreads] = e[u] >> a.page_log2;
+      const int64_t i = i0 + (int64_t)u * gthreads;
+      if (have[u] && (e[u] < 0 || (e[u] & (P - 1)))) watchdog_set(kWdBadSlot);
+      if (i < NPc) a.kv_indices[i] = e[u] >> a.page_log2;  // -1 stays -1
     }
   }
 

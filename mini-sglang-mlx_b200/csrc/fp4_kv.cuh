@@ -131,7 +131,9 @@ struct Fp4Where {
   bool have;
 };
 
-// The units of this thread, npr of them in a head row; `slots` reads go out together.
+// The units of this thread, npr of them in a head row; `slots` reads go out together. STORE: a
+// slot of -1 is a row without one, skipped; any other slot outside the pool is recorded.
+template <bool STORE>
 __device__ __forceinline__ void fp4_where(const Fp4KvArgs& a, int npr, Fp4Where (&w)[kFp4Unroll]) {
   const uint32_t half = (uint32_t)(a.Hkv * npr), per_tok = 2u * half;
   const int64_t i0 = (int64_t)blockIdx.x * (kFp4Threads * kFp4Unroll);
@@ -152,7 +154,7 @@ __device__ __forceinline__ void fp4_where(const Fp4KvArgs& a, int npr, Fp4Where 
 #pragma unroll
   for (int u = 0; u < kFp4Unroll; ++u) {
     if (w[u].slot < 0 || w[u].slot >= a.num_slots) {
-      watchdog_set(kWdBadSlot);
+      if (!STORE || w[u].slot != kNoSlot) watchdog_set(kWdBadSlot);
       w[u].slot = -1;
     }
   }
@@ -171,7 +173,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kFp4Threads) fp4_store_kernel(const Fp4KvArgs a) {
   pdl_wait_then_release();
   Fp4Where w[kFp4Unroll];
-  fp4_where(a, a.nblk, w);
+  fp4_where<true>(a, a.nblk, w);
   const int D = a.nblk * kFp4Block;
 #pragma unroll
   for (int u = 0; u < kFp4Unroll; ++u) {
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_load_kernel(const Fp4KvArgs a
   const int D = a.nblk * kFp4Block;
   const bool odd = threadIdx.x & 1;
   Fp4Where w[kFp4Unroll];
-  fp4_where(a, a.nblk, w);
+  fp4_where<false>(a, a.nblk, w);
   uint2 c[kFp4Unroll];
   uint32_t sb[kFp4Unroll];
 #pragma unroll

@@ -3,7 +3,7 @@
 // Reference behaviour (python/minisgl_mlx/layers.py:45-56 and :103-109,
 // kvcache/pool.py:47-50): q and k get rotate-half RoPE (mx.fast.rope,
 // traditional=False) at their per-token positions, then the rotated k and the
-// untouched v are written to pool slots out_loc[t].
+// untouched v are written to pool slots out_loc[t] (-1: the row has none and is not stored).
 //
 // One warp owns one (token, head, kind) row; kind 0 = q, 1 = k, 2 = v. A lane
 // handles rotation pairs (i, i + rot/2) for i = lane, lane + 32, ... The pool
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256) rope_store_kernel(RopeStoreArgs a) {
     const T* src = reinterpret_cast<const T*>(a.v) + (int64_t)t * a.v_stride + (int64_t)h * a.D;
     const int64_t slot = a.out_loc[t];
     if (slot < 0 || slot >= a.num_slots) {
-      if (lane == 0) watchdog_set(kWdBadSlot);
+      if (lane == 0 && slot != kNoSlot) watchdog_set(kWdBadSlot);
       return;
     }
     T* dst = reinterpret_cast<T*>(a.v_pool) + (slot * a.Hkv + h) * a.D;
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(256) rope_store_kernel(RopeStoreArgs a) {
     const int64_t slot = a.out_loc[t];
     if (slot >= 0 && slot < a.num_slots) {
       pool_row = reinterpret_cast<T*>(a.k_pool) + (slot * a.Hkv + h) * a.D;
-    } else if (lane == 0) {
+    } else if (lane == 0 && slot != kNoSlot) {
       watchdog_set(kWdBadSlot);
     }
   }
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256, 2) rope_store_tok_kernel(RopeStoreArgs a,
   if (do_store) {
     slot = a.out_loc[t];
     if (slot < 0 || slot >= a.num_slots) {
-      if (lane == 0 && w == 0) watchdog_set(kWdBadSlot);
+      if (lane == 0 && w == 0 && slot != kNoSlot) watchdog_set(kWdBadSlot);
       slot = -1;
     }
   }

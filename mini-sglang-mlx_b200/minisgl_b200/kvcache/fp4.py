@@ -95,7 +95,8 @@ class FP4KVCache:
         return row if T > 1 else H * D
 
     def store_kv(self, k: torch.Tensor, v: torch.Tensor, out_loc: torch.Tensor, layer_id: int) -> None:
-        """Quantise k/v ``[T, Hkv, D]`` into slots ``out_loc`` ``[T]`` (unique; token rows may be strided)."""
+        """Quantise k/v ``[T, Hkv, D]`` into slots ``out_loc`` ``[T]`` (unique, or -1: the row is skipped;
+        token rows may be strided)."""
         T = self._slots(out_loc)
         ks, vs = self._rows("k", k, T), self._rows("v", v, T)
         index = self.device.index

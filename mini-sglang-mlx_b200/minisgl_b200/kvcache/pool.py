@@ -75,7 +75,10 @@ class MHAKVCache:
         return self.v[layer_id]
 
     def store_kv(self, k: torch.Tensor, v: torch.Tensor, out_loc: torch.Tensor, layer_id: int) -> None:
-        """Write k/v ``[T, Hkv, D]`` into slots ``out_loc`` ``[T]`` (kvcache/pool.py:47-50)."""
+        """Write k/v ``[T, Hkv, D]`` into slots ``out_loc`` ``[T]`` (kvcache/pool.py:47-50).
+
+        Slots are unique, or -1: that row is skipped.
+        """
         T = k.shape[0]
         assert k.shape == v.shape == (T, self.num_kv_heads, self.head_dim), (k.shape, v.shape)
         assert k.dtype == v.dtype == self.dtype

@@ -1,0 +1,173 @@
+"""Device-built prefill tables (b2a_extend_metadata) where a batch is smaller than its buffers, does
+not fit them or names rows that do not exist: what a store and an attention call behind them do.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+
+from helpers import HeadConfig, rand, to_dev, torch_dtype
+from minisgl_b200 import workloads as W
+
+pytestmark = pytest.mark.gpu
+
+HQ, HKV, D, P = 16, 8, 128, 16
+
+
+def _device_error() -> int:
+    import torch
+
+    from minisgl_b200 import _native as nat
+
+    code = ctypes.c_int(-1)
+    nat.call("b2a_device_error", torch.cuda.current_stream().cuda_stream, ctypes.byref(code))
+    return code.value
+
+
+def _i32(a):
+    import torch
+
+    return torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).cuda()
+
+
+def _cache(pool, n, dtype="bfloat16"):
+    from minisgl_b200 import FP4KVCache, MHAKVCache
+
+    return (FP4KVCache if pool == "fp4" else MHAKVCache)(1, n, HKV, D, torch_dtype(dtype), "cuda")
+
+
+def _backend(lens, pool="fp4", dtype="bfloat16"):
+    from minisgl_b200 import B200AttnBackend
+
+    lens = np.asarray(lens)
+    rng = np.random.default_rng(int(lens.sum()))
+    pb = W.allocate_pages(lens, (int(((lens + P - 1) // P).sum()) + 4) * P, P, rng)
+    cache = _cache(pool, pb.num_slots, dtype)
+    return B200AttnBackend(HeadConfig(HQ, HKV, D), cache, pb.page_table, P), pb, rng
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("pool", ["fp4", "dense"])
+def test_a_captured_step_stores_its_own_batch_only(pool, dtype):
+    """Tables, store and extend captured once at full capacity: a replay with fewer tokens leaves
+    every other slot of the pool as it was, byte for byte, and attends as the eager call does."""
+    import torch
+
+    cap = np.array([200, 96, 40, 130])
+    be, pb, rng = _backend(cap, pool, dtype)
+    cache, T = be.kv_cache, int(cap.sum())
+    meta = be.alloc_extend_metadata(4, T, int(((cap + P - 1) // P).sum()))
+    table, rows = _i32(pb.page_table), _i32(pb.rows)
+    cached, lens = _i32(np.zeros(4)), _i32(cap)
+    q = torch.zeros(T, HQ, D, dtype=torch_dtype(dtype), device="cuda")
+    k = torch.zeros(T, HKV, D, dtype=torch_dtype(dtype), device="cuda")
+    v = torch.zeros_like(k)
+
+    def step():
+        be.build_extend_metadata_device(meta, table, rows, cached, lens)
+        cache.store_kv(k, v, meta.out_loc, 0)
+        return be._forward_prefill(q, None, None, 0, meta)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    done = np.zeros(4, np.int64)
+    for upto in ([200, 96, 3, 130], [200, 96, 40, 130], [200, 96, 40, 130]):
+        upto = np.array(upto)
+        ext = upto - done
+        if not ext.any():  # a second pass over the last request's last tokens
+            done = upto - np.array([0, 0, 0, 7])
+            ext = upto - done
+        n = int(ext.sum())
+        for t, h in ((q, HQ), (k, HKV), (v, HKV)):
+            t.copy_(to_dev(rand(rng, (T, h, D), dtype), dtype))
+        cached.copy_(_i32(done))
+        lens.copy_(_i32(upto))
+        before = cache.buffer.clone()
+        loc = pb.page_table[np.repeat(pb.rows, ext), np.concatenate([np.arange(a, b) for a, b in zip(done, upto)])]
+        g.replay()
+        torch.cuda.synchronize()
+        got = out[:n].clone()
+        np.testing.assert_array_equal(meta.out_loc[:n].cpu().numpy(), loc)
+        assert (meta.out_loc[n:] == -1).all()
+        changed = cache.buffer[0] != before[0]
+        changed = changed.any(-1) if pool == "fp4" else changed.any(0).flatten(1).any(-1)
+        others = np.setdiff1d(np.arange(pb.num_slots), loc)
+        assert not changed[torch.from_numpy(others).cuda()].any(), "a slot of another batch was written"
+        host = be.extend_metadata_from_lens(pb.rows, upto, ext)
+        cache.store_kv(k[:n], v[:n], _i32(loc), 0)
+        assert bool((be._forward_prefill(q[:n], None, None, 0, host) == got).all())
+        done = upto
+    assert _device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_stores_skip_rows_without_a_slot(dtype):
+    """Slot -1 is padding: not stored, not an error; any other slot outside the pool is one."""
+    import torch
+
+    from minisgl_b200.config import RotaryConfig
+    from minisgl_b200.layers import RotaryEmbedding
+
+    rng = np.random.default_rng(3)
+    k, v = (to_dev(rand(rng, (4, HKV, D), dtype), dtype) for _ in range(2))
+    q = to_dev(rand(rng, (4, HQ, D), dtype), dtype)
+    rope = RotaryEmbedding(RotaryConfig(D, D, 1e6, 4096))
+    pos = _i32(np.arange(4))
+    for pool in ("fp4", "dense"):
+        for call in ("store", "rope"):
+            for loc, code in (([5, -1, 2, -1], 0), ([5, -2, 2, -1], 32), ([5, 16, 2, -1], 32)):
+                cache = _cache(pool, 16, dtype)
+                if call == "store":
+                    cache.store_kv(k, v, _i32(loc), 0)
+                else:
+                    rope.rope_store_(q.clone(), k.clone(), v, pos, _i32(loc), cache, 0)
+                assert _device_error() == code, (pool, call, loc)
+                used = cache.rows(0).any(-1) if pool == "fp4" else cache.v_cache(0).flatten(1).any(-1)
+                assert torch.nonzero(used).flatten().tolist() == [2, 5]
+
+
+def test_no_slot_is_left_from_an_earlier_batch():
+    """Rows outside the table and batches that do not fit: their slots are -1, whatever the buffers held."""
+    lens, cached = np.array([40, 33, 64]), np.array([8, 0, 60])
+    be, pb, _ = _backend(lens)
+    T, NP = int((lens - cached).sum()), int(((lens + P - 1) // P).sum())
+    table = _i32(pb.page_table)
+    pos = np.concatenate([np.arange(c, n) for c, n in zip(cached, lens)])
+    req = np.repeat(np.arange(3), lens - cached)
+    loc = pb.page_table[pb.rows[req], pos]
+    for bad in (-1, 99):  # a request whose row does not exist
+        meta = be.alloc_extend_metadata(3, T + 9, NP + 3)
+        meta.out_loc.fill_(7)
+        meta.kv_indices.fill_(1)
+        rows = pb.rows.copy()
+        rows[1] = bad
+        be.build_extend_metadata_device(meta, table, _i32(rows), _i32(cached), _i32(lens))
+        assert _device_error() == 34
+        np.testing.assert_array_equal(meta.out_loc.cpu().numpy(), np.concatenate([np.where(req == 1, -1, loc), [-1] * 9]))
+        pages = meta.kv_indices.cpu().numpy()
+        assert (pages[3:6] == -1).all() and (pages[[0, 1, 2, 6, 7, 8, 9]] >= 0).all() and (pages[10:] == 1).all()
+    for t, p in ((T - 1, NP), (T, NP - 1)):  # a capacity one short
+        meta = be.alloc_extend_metadata(3, t, p)
+        meta.out_loc.fill_(7)
+        be.build_extend_metadata_device(meta, table, _i32(pb.rows), _i32(cached), _i32(lens))
+        assert _device_error() == 34
+        assert (meta.out_loc == -1).all() and (meta.work == 0).all()
+
+
+def test_negative_slots_of_the_table_are_reported():
+    """An entry of the page table that was never filled is an error, not padding."""
+    be, pb, _ = _backend([40])
+    table = pb.page_table.copy()
+    table[0, 21] = -1
+    meta = be.alloc_extend_metadata(1, 40, 3)
+    be.build_extend_metadata_device(meta, _i32(table), _i32([0]), _i32([0]), _i32([40]))
+    assert _device_error() == 32
