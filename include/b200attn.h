@@ -462,7 +462,9 @@ int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int
  *   work          : out int32 [work_capacity * 4], b2a_extend_plan's list for
  *                   tile_q (at most 256), then empty tiles {0, 0, 0, 0}; 16-byte
  *                   aligned; min(B, T) + T / tile_q entries are always enough
- *   counts        : out int32 [2] = {new tokens, tiles}
+ *   counts        : out int32 [2] = {new tokens, tiles}; tiles is 0 for a batch
+ *                   that does not fit, and both are 0 (with all-zero indptr) for one
+ *                   of more than 2^31 - 1 tokens or pages or 2^24 tiles
  * Identical values to the host builders. Entries past what the batch needs are
  * left as they were, except work and out_loc: every entry of out_loc behind the
  * last token is -1, so that a store of all q_capacity rows (a captured step)

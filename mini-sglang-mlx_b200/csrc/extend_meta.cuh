@@ -153,12 +153,20 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
       }
       small = small && all <= (c == 2 ? (long long)kEmMaxWork : 0x7fffffffll);
     }
-    if (!small) {  // the same on every thread: an empty work list, the other tables as they were
+    if (!small) {  // the same on every thread: the tables of a batch without tokens
       if (blockIdx.x == 0 && tid == 0) watchdog_set(kWdMetaOverflow);
       for (int i = blockIdx.x * kEmThreads + tid; i < a.work_capacity; i += gridDim.x * kEmThreads)
         reinterpret_cast<int4*>(a.work)[i] = make_int4(0, 0, 0, 0);
       for (int64_t i = (int64_t)blockIdx.x * kEmThreads + tid; i < a.q_capacity; i += (int64_t)gridDim.x * kEmThreads)
         a.out_loc[i] = kNoSlot;
+      for (int b = blockIdx.x * kEmThreads + tid; b <= B; b += gridDim.x * kEmThreads) {
+        a.qo_indptr[b] = a.kv_indptr[b] = 0;
+        if (b < B) {
+          a.last_indices[b] = -1;
+          a.last_page_len[b] = 0;
+        }
+      }
+      if (blockIdx.x == 0 && tid < 2) a.counts[tid] = 0;
       return;
     }
     for (int b = b0; b < b1; ++b) {
@@ -183,7 +191,7 @@ __global__ void __launch_bounds__(kEmThreads) extend_meta_kernel(const ExtendMet
     a.qo_indptr[b] = qo[b];
     a.kv_indptr[b] = kv[b];
     if (b < B) {
-      a.last_indices[b] = qo[b + 1] - 1;
+      a.last_indices[b] = (int)min((int64_t)qo[b + 1], a.q_capacity) - 1;  // inside the buffer, fits or not
       const int np = kv[b + 1] - kv[b];
       a.last_page_len[b] = np > 0 ? cached[b] + (qo[b + 1] - qo[b]) - ((np - 1) << a.page_log2) : 0;
     }

@@ -171,3 +171,33 @@ def test_negative_slots_of_the_table_are_reported():
     meta = be.alloc_extend_metadata(1, 40, 3)
     be.build_extend_metadata_device(meta, _i32(table), _i32([0]), _i32([0]), _i32([40]))
     assert _device_error() == 32
+
+
+def test_a_batch_past_the_counters_leaves_no_table():
+    """8,192 requests of 300,000 new tokens: their sum passes 2^31, and nothing is left of the batch before."""
+    import torch
+
+    B, L = 8192, 300_000
+    be, pb, _ = _backend([40])
+    table = torch.zeros(1, L, dtype=torch.int32, device="cuda")  # all requests share a row: no entry is read
+    meta = be.alloc_extend_metadata(B, 64, 64)
+    rows, cached, lens = (torch.zeros(B, dtype=torch.int32, device="cuda") for _ in range(3))
+    lens[5] = 9
+    be.build_extend_metadata_device(meta, table, rows, cached, lens)
+    assert _device_error() == 0 and meta.counts.tolist() == [9, 1]
+    lens.fill_(L)
+    be.build_extend_metadata_device(meta, table, rows, cached, lens)
+    assert _device_error() == 34
+    assert meta.counts.tolist() == [0, 0]
+    for t in (meta.work, meta.qo_indptr, meta.kv_indptr, meta.kv_last_page_len):
+        assert (t == 0).all()
+    assert (meta.out_loc == -1).all() and (meta.last_indices == -1).all()
+
+
+def test_last_indices_stay_inside_a_buffer_that_is_too_small():
+    """A gather of the last tokens behind a batch that does not fit reads rows that exist."""
+    be, pb, _ = _backend([40, 33])
+    meta = be.alloc_extend_metadata(2, 50, 6)
+    be.build_extend_metadata_device(meta, _i32(pb.page_table), _i32(pb.rows), _i32([0, 0]), _i32([40, 33]))
+    assert _device_error() == 34
+    assert meta.last_indices.tolist() == [39, 49]
