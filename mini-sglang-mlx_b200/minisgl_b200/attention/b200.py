@@ -111,6 +111,7 @@ class B200AttnBackend(BaseAttnBackend):
         self._stager = PinnedStager()
         self._workspace = torch.empty(0, dtype=torch.uint8, device=self.device)
         self._stage: tuple | None = None  # packed K/V staging pools for small-page prefill
+        self._tiles: dict = {}  # page size -> query tokens of an extend tile
         self.fp4 = isinstance(kv_cache, FP4KVCache)  # the pool holds 4-bit rows (kvcache/fp4.py)
         n = nat.ctypes.c_int(0)
         with torch.cuda.device(self.device):
@@ -326,7 +327,7 @@ class B200AttnBackend(BaseAttnBackend):
         capacity of a batch whose lengths are known on the device only (a captured step). A batch
         that needs less leaves the tails of ``positions`` and ``kv_indices`` as they were, -1 (no slot:
         ``store_kv`` skips the row) in the tail of ``out_loc``, and empty tiles at the end of ``work``. ``tile_q`` defaults to the tile of this
-        backend's extend kernel. Host copies of ``cached`` and ``lens``, where the caller has
+        backend's extend kernel; tables of a larger one serve other consumers, ``forward`` refuses them. Host copies of ``cached`` and ``lens``, where the caller has
         them, let a 4-bit pool cut long requests' keys into runs as evenly as
         ``extend_metadata_from_lens`` does; without them it assumes requests of equal length.
         """
@@ -423,6 +424,12 @@ class B200AttnBackend(BaseAttnBackend):
     def _forward_prefill(self, q, k, v, layer_id: int, meta: B200PrefillMetadata) -> torch.Tensor:
         T = meta.total_q
         assert q.shape == (T, self.Hq, self.D), q.shape
+        if meta.tile_q:  # tables built on the device, for a tile the caller may have chosen
+            tile = self._tiles.get(meta.page_size)
+            if tile is None:
+                tile = self._tiles[meta.page_size] = self._tile_q(meta.page_size)
+            if meta.tile_q > tile:  # the kernel would cut every tile at its own size
+                raise ValueError(f"prefill tables in tiles of {meta.tile_q} tokens: this extend takes at most {tile}")
         q = self._query(q)
         out = torch.empty_like(q)
         B = meta.qo_indptr.numel() - 1

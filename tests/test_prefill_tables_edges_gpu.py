@@ -201,3 +201,27 @@ def test_last_indices_stay_inside_a_buffer_that_is_too_small():
     be.build_extend_metadata_device(meta, _i32(pb.page_table), _i32(pb.rows), _i32([0, 0]), _i32([40, 33]))
     assert _device_error() == 34
     assert meta.last_indices.tolist() == [39, 49]
+
+
+@pytest.mark.parametrize("pool", ["fp4", "dense"])
+def test_tables_of_too_large_tiles_are_refused(pool):
+    """The kernel would leave the rows past its own tile unwritten; smaller tiles give the same rows."""
+    lens = np.array([300, 90])
+    be, pb, rng = _backend(lens, pool)
+    x = to_dev(rand(rng, (pb.num_slots, HKV, D), "bfloat16"), "bfloat16")
+    be.kv_cache.store_kv(x, x, _i32(np.arange(pb.num_slots)), 0)
+    q = to_dev(rand(rng, (390, HQ, D), "bfloat16"), "bfloat16")
+    tile = be._tile_q(P)
+    got = {}
+    for t in (None, tile // 2, 16, tile + 1, 256):
+        meta = be.alloc_extend_metadata(2, 390, 25, tile_q=t)
+        be.build_extend_metadata_device(meta, _i32(pb.page_table), _i32(pb.rows), _i32([0, 0]), _i32(lens))
+        if t is not None and t > tile:
+            with pytest.raises(ValueError, match="tile"):
+                be._forward_prefill(q, None, None, 0, meta)
+        else:
+            got[t] = be._forward_prefill(q, None, None, 0, meta).float()
+    # either output: weights rounded to bf16 at worst (2^-8 of the values they weigh), one bf16 rounding (2^-8)
+    for t in (tile // 2, 16):
+        assert (got[t] - got[None]).abs().max() <= 2 * 2.0 ** -7 * x.float().abs().max()
+    assert _device_error() == 0
