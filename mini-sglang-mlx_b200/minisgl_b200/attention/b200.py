@@ -313,6 +313,8 @@ class B200AttnBackend(BaseAttnBackend):
     PACK_PAGE = 16
 
     # ------------------------------------------------------------ prefill metadata built on the device
+    MAX_DEVICE_EXTEND = 8192  # requests of b2a_extend_metadata; the host builders take any number
+
     @property
     def device_extend(self) -> bool:
         """Whether this pool's extend takes tables built on the device (else: host-built key groups)."""

@@ -213,7 +213,9 @@ class Scheduler(HostScheduler):
 
     def _prepare(self, batch: Batch) -> None:
         reqs = batch.reqs
-        if batch.is_prefill and self.engine.page_table_dev is not None and self.engine.attn_backend.device_extend:
+        be = self.engine.attn_backend
+        if (batch.is_prefill and self.engine.page_table_dev is not None and be.device_extend
+                and len(reqs) <= be.MAX_DEVICE_EXTEND):
             self._prepare_prefill_device(batch)
             return
         positions, out_loc = batch_positions_out_loc(batch, self.engine.page_table)
