@@ -56,11 +56,12 @@ def paged_kv_indices(
         first = page_table[rows[:, None], cols[None, :]]
         kv_indices = first[valid] // P
         if check:
-            _check_page_runs(page_table, rows, lens, P)
+            check_page_runs(page_table, rows, lens, P)
     return kv_indptr, np.ascontiguousarray(kv_indices, dtype=np.int32), last_page_len
 
 
-def _check_page_runs(page_table: np.ndarray, rows: np.ndarray, lens: np.ndarray, P: int) -> None:
+def check_page_runs(page_table: np.ndarray, rows: np.ndarray, lens: np.ndarray, P: int) -> None:
+    """ValueError unless every page of the rows' first ``lens`` tokens is an aligned run of P slots."""
     for row, n in zip(rows.tolist(), lens.tolist()):
         slots = page_table[row, :n].astype(np.int64)
         pos = np.arange(n)

@@ -29,7 +29,7 @@ import numpy as np
 import torch
 
 from ..attention import create_attention_backend, page_table_scatter
-from ..attention.base import PinnedStager
+from ..attention.base import CHECK_METADATA, PinnedStager, check_page_runs
 from ..core import Batch, Context, Req, SamplingParams, batch_positions_out_loc, set_global_ctx
 from ..kvcache import FP4KVCache, MHAKVCache
 from .graph import DecodeGraphs
@@ -259,6 +259,8 @@ class Scheduler(HostScheduler):
         rows = np.array([r.table_idx for r in reqs], dtype=np.int32)
         cached = np.array([r.cached_len for r in reqs], dtype=np.int32)
         lens = np.array([r.device_len for r in reqs], dtype=np.int32)
+        if CHECK_METADATA and self.cfg.page_size > 1:  # the kernel looks at the first slot of a page only
+            check_page_runs(self.engine.page_table, rows, lens, self.cfg.page_size)
         ids = np.concatenate([r.input_ids[r.cached_len: r.device_len] for r in reqs]).astype(np.int32)
         cols = np.concatenate([np.arange(n, dtype=np.int32) for n in lens.tolist()])
         r_tok = np.repeat(rows, lens)

@@ -47,3 +47,36 @@ def test_batches_past_the_device_tables_go_to_the_host_builder(n, where, monkeyp
     s = _scheduler(np.arange(n * 4, dtype=np.int32).reshape(n, 4))
     S.Scheduler._prepare(s, _batch([_req(b, 1) for b in range(n)]))
     assert s.engine.attn_backend.calls == [(where, n)]
+
+
+class _Tables:
+    """Stands in for the metadata that the device fills."""
+
+    positions = out_loc = "device"
+
+
+def _device_scheduler(table, monkeypatch, page_size=4):
+    s = _scheduler(table, page_size)
+    monkeypatch.setattr(S, "page_table_scatter", lambda *a: None)
+    be = s.engine.attn_backend
+    be.alloc_extend_metadata = lambda *a, **kw: be.calls.append((a, kw)) or _Tables()
+    be.build_extend_metadata_device = lambda *a: None
+    return s
+
+
+@pytest.mark.parametrize("bad", [None, "broken run", "slot of another page"])
+def test_the_metadata_check_covers_device_built_tables(bad, monkeypatch):
+    """Every page has to be an aligned run of slots, also where its first slot, all the kernel sees, is right."""
+    table = np.concatenate([np.arange(8, 16), np.arange(32, 40)]).astype(np.int32).reshape(2, 8)
+    if bad == "broken run":
+        table[1, 5:7] = table[1, [6, 5]]
+    elif bad:
+        table[0, 5] = 60
+    s = _device_scheduler(table, monkeypatch)
+    monkeypatch.setattr(S, "CHECK_METADATA", True, raising=False)
+    batch = _batch([_req(0, 6, 2), _req(1, 8)])
+    if bad is None:
+        S.Scheduler._prepare_prefill_device(s, batch)
+    else:
+        with pytest.raises(ValueError, match="aligned runs"):
+            S.Scheduler._prepare_prefill_device(s, batch)
