@@ -65,7 +65,8 @@ class B200PrefillMetadata:
     pack: "PackPlan | None" = None
     group_starts: bool = False
     # set by alloc_extend_metadata (device-built metadata): the new tokens' positions and pool
-    # slots, and int32 [2] new tokens, tiles; q_offsets is then empty
+    # slots, and int32 [2] new tokens, tiles; q_offsets is then empty, until a caller who knows the
+    # lengths on the host fills it
     positions: torch.Tensor | None = None
     out_loc: torch.Tensor | None = None
     counts: torch.Tensor | None = None

@@ -270,6 +270,7 @@ class Scheduler(HostScheduler):
         P = self.cfg.page_size
         meta = be.alloc_extend_metadata(len(reqs), len(ids), int(((lens + P - 1) // P).sum()), cached=cached, lens=lens)
         be.build_extend_metadata_device(meta, self.engine.page_table_dev, dev[0], dev[1], dev[2])
+        meta.q_offsets = np.concatenate([[0], np.cumsum(lens - cached)]).tolist()
         batch.positions, batch.out_loc, batch.rows, batch.input_ids = meta.positions, meta.out_loc, dev[0], dev[3]
         batch.attn_metadata = meta
 

@@ -80,3 +80,11 @@ def test_the_metadata_check_covers_device_built_tables(bad, monkeypatch):
     else:
         with pytest.raises(ValueError, match="aligned runs"):
             S.Scheduler._prepare_prefill_device(s, batch)
+
+
+def test_device_built_tables_keep_the_host_offsets(monkeypatch):
+    """q_offsets, a field of the prefill metadata that a model may read, as the host builder gives it."""
+    s = _device_scheduler(np.arange(24, dtype=np.int32).reshape(3, 8), monkeypatch)
+    batch = _batch([_req(0, 6, 2), _req(1, 8), _req(2, 7, 6)])
+    S.Scheduler._prepare_prefill_device(s, batch)
+    assert batch.attn_metadata.q_offsets == [0, 4, 12, 13]
