@@ -252,6 +252,7 @@ __global__ void __launch_bounds__(kTc2Threads, 1)
   const int r = w.x, tb = w.y;
   const int nq = min(w.z, 2 * TT);
   if (w.z > nq && threadIdx.x == 0) watchdog_set(kWdTileTooLarge);
+  if (nq <= 0) return;  // unused entry behind a device-built work list
   const int nq_t[2] = {min(nq, TT), max(0, nq - TT)};
   const int h = blockIdx.x;
   const int P = 1 << a.page_log2;

@@ -322,8 +322,13 @@ class B200AttnBackend(BaseAttnBackend):
         P = self.page_size
         return self.fp4 or P >= self.PACK_PAGE or self._tile_q(P) == self._tile_q(self.PACK_PAGE)
 
+    def extend_tiles(self, cached: np.ndarray, lens: np.ndarray) -> int:
+        """Work items of an extend over requests of ``lens`` tokens, ``cached`` of them in the pool."""
+        return int((-(-(np.asarray(lens) - np.asarray(cached)) // self._tile_q(self.page_size))).sum())
+
     def alloc_extend_metadata(self, batch_size: int, total_q: int, total_pages: int, tile_q: int | None = None,
-                              cached: np.ndarray | None = None, lens: np.ndarray | None = None) -> B200PrefillMetadata:
+                              cached: np.ndarray | None = None, lens: np.ndarray | None = None,
+                              n_work: int | None = None) -> B200PrefillMetadata:
         """Prefill metadata of ``batch_size`` requests for ``build_extend_metadata_device`` to fill.
 
         ``total_q`` new tokens and ``total_pages`` pages in all: what the batch needs, or the
@@ -333,6 +338,8 @@ class B200AttnBackend(BaseAttnBackend):
         backend's extend kernel; tables of a larger one serve other consumers, ``forward`` refuses them. Host copies of ``cached`` and ``lens``, where the caller has
         them, let a 4-bit pool cut long requests' keys into runs as evenly as
         ``extend_metadata_from_lens`` does; without them it assumes requests of equal length.
+        ``n_work`` is the number of tiles where the caller knows it (``extend_tiles``); the default is
+        the most that ``total_q`` tokens of ``batch_size`` requests can take.
         """
         P = self.page_size
         if tile_q is None:
@@ -343,7 +350,11 @@ class B200AttnBackend(BaseAttnBackend):
         if batch_size < 1 or total_q < 0 or total_pages < 0 or tile_q < 1:
             raise ValueError(f"alloc_extend_metadata: batch {batch_size}, {total_q} tokens, {total_pages} pages, "
                              f"tile {tile_q}")
-        n_work = min(batch_size, total_q) + total_q // tile_q
+        most = min(batch_size, total_q) + total_q // tile_q
+        if n_work is None:
+            n_work = most
+        elif not 0 <= n_work <= most:
+            raise ValueError(f"alloc_extend_metadata: {n_work} tiles for {total_q} tokens in tiles of {tile_q}")
         sizes = [batch_size + 1, total_q, total_q, batch_size, batch_size + 1, total_pages, batch_size, 4 * n_work, 2]
         # one allocation, every array on a 64-byte boundary (work is written as int4)
         starts = np.cumsum([0] + [(n + 15) // 16 * 16 for n in sizes])

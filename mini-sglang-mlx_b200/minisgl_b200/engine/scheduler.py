@@ -268,7 +268,8 @@ class Scheduler(HostScheduler):
                                   self.engine.device)
         page_table_scatter(self.engine.page_table_dev, *dev[4:])
         P = self.cfg.page_size
-        meta = be.alloc_extend_metadata(len(reqs), len(ids), int(((lens + P - 1) // P).sum()), cached=cached, lens=lens)
+        meta = be.alloc_extend_metadata(len(reqs), len(ids), int(((lens + P - 1) // P).sum()), cached=cached, lens=lens,
+                                        n_work=be.extend_tiles(cached, lens))
         be.build_extend_metadata_device(meta, self.engine.page_table_dev, dev[0], dev[1], dev[2])
         meta.q_offsets = np.concatenate([[0], np.cumsum(lens - cached)]).tolist()
         batch.positions, batch.out_loc, batch.rows, batch.input_ids = meta.positions, meta.out_loc, dev[0], dev[3]

@@ -20,6 +20,9 @@ class _Backend:
     def __init__(self):
         self.calls = []
 
+    def extend_tiles(self, cached, lens):
+        return int(sum(-(-(n - c) // 3) for c, n in zip(cached, lens)))
+
     def prepare_metadata(self, batch):
         self.calls.append(("host", batch.size))
 
@@ -88,3 +91,11 @@ def test_device_built_tables_keep_the_host_offsets(monkeypatch):
     batch = _batch([_req(0, 6, 2), _req(1, 8), _req(2, 7, 6)])
     S.Scheduler._prepare_prefill_device(s, batch)
     assert batch.attn_metadata.q_offsets == [0, 4, 12, 13]
+
+
+def test_device_built_tables_hold_the_batch_s_own_tiles(monkeypatch):
+    """No empty tiles behind the work list of a batch whose lengths are known here: ceil(4/3) + ceil(8/3) + 1."""
+    s = _device_scheduler(np.arange(24, dtype=np.int32).reshape(3, 8), monkeypatch)
+    S.Scheduler._prepare_prefill_device(s, _batch([_req(0, 6, 2), _req(1, 8), _req(2, 7, 6)]))
+    (args, kw), = s.engine.attn_backend.calls
+    assert args == (3, 13, 6) and kw["n_work"] == 6

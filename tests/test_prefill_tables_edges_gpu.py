@@ -225,3 +225,27 @@ def test_tables_of_too_large_tiles_are_refused(pool):
     for t in (tile // 2, 16):
         assert (got[t] - got[None]).abs().max() <= 2 * 2.0 ** -7 * x.float().abs().max()
     assert _device_error() == 0
+
+
+@pytest.mark.parametrize("pool", ["fp4", "dense"])
+def test_work_lists_of_known_batches_are_exact(pool):
+    """With its number of tiles given, a device-built work list is the host's, without empty tiles; the
+    default list has some, which the attention call skips."""
+    lens, cached = np.array([256, 90, 17, 40]), np.array([0, 80, 16, 0])
+    be, pb, rng = _backend(lens, pool)
+    x = to_dev(rand(rng, (pb.num_slots, HKV, D), "bfloat16"), "bfloat16")
+    be.kv_cache.store_kv(x, x, _i32(np.arange(pb.num_slots)), 0)
+    T, NP = int((lens - cached).sum()), int(((lens + P - 1) // P).sum())
+    q = to_dev(rand(rng, (T, HQ, D), "bfloat16"), "bfloat16")
+    host = be.extend_metadata_from_lens(pb.rows, lens, lens - cached)
+    assert be.extend_tiles(cached, lens) == host.n_work
+    want = be._forward_prefill(q, None, None, 0, host)
+    for n_work in (host.n_work, None):
+        meta = be.alloc_extend_metadata(4, T, NP, cached=cached, lens=lens, n_work=n_work)
+        assert (meta.n_work == host.n_work) == (n_work is not None)
+        be.build_extend_metadata_device(meta, _i32(pb.page_table), _i32(pb.rows), _i32(cached), _i32(lens))
+        assert bool((be._forward_prefill(q, None, None, 0, meta) == want).all())
+    assert _device_error() == 0
+    for bad in (-1, T + 5):
+        with pytest.raises(ValueError, match="tiles"):
+            be.alloc_extend_metadata(4, T, NP, n_work=bad)
