@@ -163,10 +163,11 @@ __device__ __forceinline__ void fp4_where(const Fp4KvArgs& a, int npr, Fp4Where 
 // x / s to nearest for |x| <= 2^13 and an e4m3 s > 0 with y = 1 / s to nearest: Markstein's
 // correction of x * y by its remainder ("Computation of elementary functions on the IBM RISC
 // System/6000 processor", 1990), three operations instead of a division per element. The
-// remainder is exact unless x is so small that the code is zero either way.
+// remainder is exact unless x is so small that the code is zero either way. The remainder of a
+// zero is +0 whatever its sign, which x gives back: the code keeps it.
 __device__ __forceinline__ float fp4_quotient(float x, float s, float y) {
   const float q = x * y;
-  return fmaf(fmaf(-q, s, x), y, q);
+  return copysignf(fmaf(fmaf(-q, s, x), y, q), x);
 }
 
 template <typename T, bool VEC>
