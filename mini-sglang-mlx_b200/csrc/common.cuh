@@ -14,6 +14,7 @@ namespace b2a {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kNaN = __builtin_nanf("");
 
 // Watchdog word: a bounded wait that gives up writes a nonzero code here and
 // the kernel unwinds. Read (and cleared) by b2a_device_error().

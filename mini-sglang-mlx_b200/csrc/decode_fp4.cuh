@@ -34,7 +34,9 @@
 // bits). The lazy maximum of decode_mma.cuh (it moves when a score exceeds it by
 // more than 8) is kept 7 below the score that set it: weights lie in [0, 2^15] with
 // the largest at least 2^7, so a weight that fp16 holds as a subnormal is off by
-// at most 2^-32 of the largest. Softmax statistics and accumulators are fp32.
+// at most 2^-32 of the largest. Softmax statistics and accumulators are fp32. A row that has seen a
+// key therefore sums to at least 2^7: a smaller sum comes from infinite scores, or from ones past
+// 2^27 whose rounding alone exceeds the softmax's range, and the row becomes NaN (fp4_row_lost).
 #pragma once
 
 #include "decode.cuh"
@@ -95,6 +97,9 @@ __device__ __forceinline__ void fp4_row_factor(float amax, float& f, float& inv)
   f = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
   inv = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
 }
+
+// Whether a row's weights are lost, for the weight sum of a row that has seen a key (NaN: shown already).
+__device__ __forceinline__ bool fp4_row_lost(float sum) { return sum < 1.f; }
 
 // Words of codes a lane reads from one K row (D/4 features) and one V row (D/8 features).
 template <int N>
@@ -570,7 +575,8 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const Dec
         if (c < G) {
           const size_t row = (size_t)h * G + c;
           float r[EPL];
-          const float f = slot < 0 ? (lsum[n] > 0.f ? v_scale / lsum[n] : 0.f) : v_scale;
+          float f = slot < 0 ? (lsum[n] > 0.f ? v_scale / lsum[n] : 0.f) : v_scale;
+          if (ntok > 0 && fp4_row_lost(lsum[n])) f = kNaN;
 #pragma unroll
           for (int mt = 0; mt < KS; ++mt) {
             r[2 * mt] = acc[mt][n] * f;

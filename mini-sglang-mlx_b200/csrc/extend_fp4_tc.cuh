@@ -727,6 +727,8 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
       f2_split(s01, lo, hi);
       l = l * alpha + (lo + hi);
     }
+    // a row that has seen a key in these blocks has weights, or none that hold (decode_fp4.cuh)
+    if (my_nb > 0 && live && lim_abs >= (b0 + (C::NS == 2 && !wide ? t : 0)) * KB && fp4_row_lost(l)) l = kNaN;
     // ---- epilogue
     const bool got = __all_sync(FULL, mbar_wait(mma_done, 0, kWdExtendBar));
     tc_fence_after();

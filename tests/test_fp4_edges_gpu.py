@@ -49,3 +49,131 @@ def test_negative_zero_keeps_its_sign(dtype):
     assert np.signbit(k[k == 0]).sum() > 100
     np.testing.assert_array_equal(c.rows(0).cpu().numpy(), F.pack_rows(k, -k))
     assert _device_error() == 0
+
+
+class Pool:
+    """A filled pool, its page table and its rows' exact values."""
+
+    def __init__(self, lens, Hkv, D, dtype, P, seed, gk=1.0, gv=1.0, k=None, v=None):
+        from minisgl_b200 import FP4KVCache
+
+        self.rng = rng = np.random.default_rng(seed)
+        lens = np.asarray(lens, dtype=np.int64)
+        n = int(((lens + P - 1) // P).sum() + 3) * P
+        self.pb = W.allocate_pages(lens, n, P, rng)
+        k = rand(rng, (n, Hkv, D), dtype) if k is None else np.broadcast_to(k, (n, Hkv, D)).astype(np.float32)
+        v = rand(rng, (n, Hkv, D), dtype) if v is None else np.broadcast_to(v, (n, Hkv, D)).astype(np.float32)
+        kd, vd = to_dev(k * np.float32(gk), dtype), to_dev(v * np.float32(gv), dtype)
+        self.cache = FP4KVCache(1, n, Hkv, D, torch_dtype(dtype), "cuda", k_scale=gk, v_scale=gv)
+        self.cache.store_kv(kd, vd, _i32(np.arange(n)), 0)
+        self.k = F.roundtrip(kd.double().cpu().numpy(), gk)
+        self.v = F.roundtrip(vd.double().cpu().numpy(), gv)
+
+    def of(self, b):
+        s = self.pb.page_table[b, : int(self.pb.lens[b])]
+        return self.k[s], self.v[s]
+
+
+def _check(got, refs, dtype, D, L, rows=slice(None)):
+    got = got.double().cpu().numpy()
+    ref, A, X, S = (np.concatenate(x) for x in zip(*refs))
+    err, tol = np.abs(got - ref)[rows], F.tolerance(ref, A, X, S, dtype, D, L)[rows]
+    assert np.isfinite(got[rows]).all()
+    assert (err <= tol).all(), (err - tol).max()
+
+
+def _refs(p, q, lens, ext, scale):
+    refs, o = [], 0
+    with np.errstate(invalid="ignore"):
+        for b, (L, n) in enumerate(zip(lens, ext)):
+            refs.append(F.attend(q[o:o + n], *p.of(b), scale, L - n))
+            o += n
+    return refs
+
+
+# what a query row holds -> nothing but NaN may come out of its heads, and nothing else changes
+BAD_QUERIES = {"nan": np.nan, "inf": np.inf, "-inf": -np.inf}
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("what", BAD_QUERIES)
+@pytest.mark.parametrize("keys", ["ones", "random"])
+def test_infinite_and_nan_queries_show_in_decode(what, keys, dtype):
+    """Over keys that are all ones, -inf makes every score -inf and +inf every score +inf: softmax has no
+    value either way. Requests of one token, of part of a step, of whole steps, and split over CTAs."""
+    from minisgl_b200 import B200AttnBackend
+
+    Hq, Hkv, D = 4, 2, 128
+    lens = [1, 15, 64, 130, 2500, 40]
+    p = Pool(lens, Hkv, D, dtype, 16, seed=3, k=1.0 if keys == "ones" else None)
+    q = rand(p.rng, (len(lens), Hq, D), dtype)
+    bad = np.zeros((len(lens), Hq), bool)
+    bad[:5, 1] = bad[3] = True  # the last request, and most heads, stay as they are
+    q[bad, 17] = BAD_QUERIES[what]
+    be = B200AttnBackend(HeadConfig(Hq, Hkv, D), p.cache, p.pb.page_table, 16)
+    good = np.where(bad[..., None], 0, q)
+    refs = _refs(p, good.astype(np.float64), lens, [1] * len(lens), be.scale)
+    for nc in (None, 1, 31):
+        out = be.forward_decode(to_dev(q, dtype), 0, be.decode_metadata_from_lens(p.pb.rows, p.pb.lens, num_ctas=nc))
+        assert np.isnan(out.double().cpu().numpy()[bad]).all(), (what, nc)
+        _check(out, refs, dtype, D, max(lens), rows=~bad)
+    assert _device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("what", BAD_QUERIES)
+@pytest.mark.parametrize("keys", ["ones", "random"])
+@pytest.mark.parametrize("D", [128, 256])
+def test_infinite_and_nan_queries_show_in_extend(D, keys, what, dtype):
+    """The same for extend: tiles of one and of two streams, a row with one visible key, a prompt in runs."""
+    from minisgl_b200 import B200AttnBackend
+
+    Hq, Hkv = 4, 2
+    lens, ext = np.array([1, 200, 90, 700]), np.array([1, 200, 3, 9])
+    p = Pool(lens, Hkv, D, dtype, 16, seed=5, k=1.0 if keys == "ones" else None)
+    q = rand(p.rng, (int(ext.sum()), Hq, D), dtype)
+    bad = np.zeros(q.shape[:2], bool)
+    bad[[0, 1, 2, 130, 200, 202, 212], 1] = bad[77] = True
+    q[bad, 17] = BAD_QUERIES[what]
+    be = B200AttnBackend(HeadConfig(Hq, Hkv, D), p.cache, p.pb.page_table, 16)
+    refs = _refs(p, np.where(bad[..., None], 0, q).astype(np.float64), lens, ext, be.scale)
+    for runs in (None, 128):
+        meta = be.extend_metadata_from_lens(p.pb.rows, lens, ext)
+        _force_runs(be, meta, runs, 6)
+        out = be._forward_prefill(to_dev(q, dtype), None, None, 0, meta)
+        assert np.isnan(out.double().cpu().numpy()[bad]).all(), (what, runs)
+        _check(out, refs, dtype, D, int(lens.max()), rows=~bad)
+    assert _device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_scores_past_the_softmax_s_range_are_never_a_silent_zero(dtype):
+    """Scores of about 2^40: fp32 rounds them by 2^16, so a row has no weights that mean anything. Values
+    are at least 1, so an output of 0 would be a row whose weights vanished unseen."""
+    from minisgl_b200 import B200AttnBackend
+
+    Hq, Hkv, D = 16, 8, 128
+    lens, ext = np.array([40, 300, 2500, 130]), np.array([40, 9, 64, 130])
+    p = Pool(lens, Hkv, D, dtype, 16, seed=6, v=2.0)
+    q = rand(p.rng, (int(ext.sum()), Hq, D), dtype) * np.float32(2.0 ** 37)
+    be = B200AttnBackend(HeadConfig(Hq, Hkv, D), p.cache, p.pb.page_table, 16)
+    last = np.cumsum(ext) - 1
+    for nc in (None, 1, 31):
+        out = be.forward_decode(to_dev(q[last], dtype), 0, be.decode_metadata_from_lens(p.pb.rows, p.pb.lens, num_ctas=nc))
+        assert not (out == 0).any()
+    for runs in (None, 256):
+        meta = be.extend_metadata_from_lens(p.pb.rows, lens, ext)
+        _force_runs(be, meta, runs, 10)
+        assert not (be._forward_prefill(to_dev(q, dtype), None, None, 0, meta) == 0).any()
+    assert _device_error() == 0
+
+
+def _force_runs(be, meta, run_keys, n_split):
+    """The same work items with their keys in runs of run_keys (None: whole)."""
+    import torch
+
+    from minisgl_b200 import _native as nat
+
+    meta.run_keys, meta.n_split = (0, 1) if run_keys is None else (run_keys, n_split)
+    n = int(nat.LIB.b2a_fp4_extend_workspace_bytes(meta.n_work, meta.n_split, be.Hkv, be.D))
+    meta.workspace = torch.zeros(n, dtype=torch.uint8, device="cuda") if n else None
