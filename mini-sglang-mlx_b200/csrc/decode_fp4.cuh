@@ -101,6 +101,12 @@ __device__ __forceinline__ void fp4_row_factor(float amax, float& f, float& inv)
 // Whether a row's weights are lost, for the weight sum of a row that has seen a key (NaN: shown already).
 __device__ __forceinline__ bool fp4_row_lost(float sum) { return sum < 1.f; }
 
+// Softmax scale of a head row's raw scores, kept above zero: at the smallest normal float every score
+// (raw ones stay below 2^35) is nothing already, while zero times a masked -inf would be NaN.
+__device__ __forceinline__ float fp4_score_scale(float inv, float qscale) {
+  return fmaxf(inv * qscale, 0x1p-126f);
+}
+
 // Words of codes a lane reads from one K row (D/4 features) and one V row (D/8 features).
 template <int N>
 __device__ __forceinline__ void fp4_lds(const uint8_t* p, uint32_t (&w)[N]) {
@@ -471,7 +477,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const Dec
           }
         }
       }
-      inv *= a.qscale;
+      inv = fp4_score_scale(inv, a.qscale);
       qs[0] = __shfl_sync(FULL, inv, 8 * t);      // column 2t
       qs[1] = __shfl_sync(FULL, inv, 8 * t + 4);  // column 2t + 1
     }

@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
           }
         }
         fp4_row_factor(amax, f, inv);
-        if (ch == 0) qfac[tile * 128 + rw] = inv * a.qscale;
+        if (ch == 0) qfac[tile * 128 + rw] = fp4_score_scale(inv, a.qscale);
         uint32_t u[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

@@ -177,3 +177,25 @@ def _force_runs(be, meta, run_keys, n_split):
     meta.run_keys, meta.n_split = (0, 1) if run_keys is None else (run_keys, n_split)
     n = int(nat.LIB.b2a_fp4_extend_workspace_bytes(meta.n_work, meta.n_split, be.Hkv, be.D))
     meta.workspace = torch.zeros(n, dtype=torch.uint8, device="cuda") if n else None
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("amp,gk", [(2.0 ** -80, 2.0 ** -100), (2.0 ** -100, 2.0 ** -30), (2.0 ** 60, 2.0 ** -100)])
+def test_scores_below_fp32_weigh_all_keys_alike(amp, gk, dtype):
+    from minisgl_b200 import B200AttnBackend
+
+    Hq, Hkv, D = 4, 2, 128
+    lens, ext = np.array([140, 9, 300, 700]), np.array([60, 1, 64, 2])  # rows that see a part of the blocks
+    p = Pool(lens, Hkv, D, dtype, 16, seed=8, gk=gk)
+    q = rand(p.rng, (int(ext.sum()), Hq, D), dtype) * np.float32(amp)
+    be = B200AttnBackend(HeadConfig(Hq, Hkv, D), p.cache, p.pb.page_table, 16)
+    last = np.cumsum(ext) - 1
+    refs = _refs(p, q[last].astype(np.float64), lens, [1] * 4, be.scale)
+    out = be.forward_decode(to_dev(q[last], dtype), 0, be.decode_metadata_from_lens(p.pb.rows, p.pb.lens))
+    _check(out, refs, dtype, D, 700)
+    refs = _refs(p, q.astype(np.float64), lens, ext, be.scale)
+    for runs in (None, 128):
+        meta = be.extend_metadata_from_lens(p.pb.rows, lens, ext)
+        _force_runs(be, meta, runs, 6)
+        _check(be._forward_prefill(to_dev(q, dtype), None, None, 0, meta), refs, dtype, D, 700)
+    assert _device_error() == 0
