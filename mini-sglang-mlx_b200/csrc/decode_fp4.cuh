@@ -581,19 +581,22 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) decode_fp4_kernel(const Dec
         if (c < G) {
           const size_t row = (size_t)h * G + c;
           float r[EPL];
-          float f = slot < 0 ? (lsum[n] > 0.f ? v_scale / lsum[n] : 0.f) : v_scale;
+          // the sums reach 2^57 (2^31 weights of 2^15 and values of 2688): a row is divided before it
+          // is scaled, and a partial row of a scale above 2^64 gives up 2^48, and so does its lsum
+          const float part = v_scale > 0x1p64f ? 0x1p-48f : 1.f;
+          float f = slot < 0 ? (lsum[n] > 0.f ? 1.f / lsum[n] : 0.f) : part;
           if (ntok > 0 && fp4_row_lost(lsum[n])) f = kNaN;
 #pragma unroll
           for (int mt = 0; mt < KS; ++mt) {
-            r[2 * mt] = acc[mt][n] * f;
-            r[2 * mt + 1] = acc[mt][2 + n] * f;
+            r[2 * mt] = acc[mt][n] * f * v_scale;
+            r[2 * mt + 1] = acc[mt][2 + n] * f * v_scale;
           }
           if (slot < 0) {
             store_vec<T, EPL>(reinterpret_cast<T*>(a.out) + ((size_t)b * a.Hq + row) * D + g * EPL, r);
           } else {
             store_vec<float, EPL>(a.ws_acc + ((size_t)slot * a.Hq + row) * D + g * EPL, r);
             if (g == 0)
-              *reinterpret_cast<float2*>(a.ws_ml + ((size_t)slot * a.Hq + row) * 2) = make_float2(mref[n], lsum[n]);
+              *reinterpret_cast<float2*>(a.ws_ml + ((size_t)slot * a.Hq + row) * 2) = make_float2(mref[n], lsum[n] * part);
           }
         }
       }

@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
     T* out = reinterpret_cast<T*>(a.out);
     if (runs == 1) {
       if (writer && ok && warp_live) {
-        const float inv = l > 0.f ? a.v_scale / l : (l == l ? 0.f : l);
+        const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // before the scale: no end of fp32 is near
         // a warp's 32 rows go through shared memory, 16-byte chunks permuted by row, so that a
         // store writes whole rows and not 16 bytes of each of 32
         constexpr int CPR = D * (int)sizeof(T) / 16;  // chunks of a row
@@ -814,16 +814,18 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
           columns(c, v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = v[i] * inv * a.v_scale;
           constexpr int CPC = 32 * (int)sizeof(T) / 16;  // chunks of 32 columns
 #pragma unroll
           for (int i = 0; i < CPC; ++i) {
             uint4 x;
             if constexpr (F32) {
-              x = make_uint4(__float_as_uint(v[4 * i] * inv), __float_as_uint(v[4 * i + 1] * inv),
-                             __float_as_uint(v[4 * i + 2] * inv), __float_as_uint(v[4 * i + 3] * inv));
+              x = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                             __float_as_uint(v[4 * i + 3]));
             } else {
-              x = make_uint4(pack_bf16x2(v[8 * i] * inv, v[8 * i + 1] * inv), pack_bf16x2(v[8 * i + 2] * inv, v[8 * i + 3] * inv),
-                             pack_bf16x2(v[8 * i + 4] * inv, v[8 * i + 5] * inv), pack_bf16x2(v[8 * i + 6] * inv, v[8 * i + 7] * inv));
+              x = make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                             pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
             }
             stage[lane * CPR + ((c * CPC + i) ^ (lane & 7))] = x;
           }
@@ -894,9 +896,9 @@ __global__ void __launch_bounds__(kF4Threads, 1) extend_fp4_tc_kernel(const F4Ar
               M = Mn;
             }
           }
-          const float inv = Ls > 0.f ? a.v_scale / Ls : (Ls != Ls ? Ls : 0.f);
+          const float inv = Ls > 0.f ? 1.f / Ls : (Ls != Ls ? Ls : 0.f);
 #pragma unroll
-          for (int e = 0; e < EPT; ++e) acc[e] *= inv;
+          for (int e = 0; e < EPT; ++e) acc[e] = acc[e] * inv * a.v_scale;
           store_vec<T, EPT>(out + ((size_t)(q0 + tb + tt * TT + tk) * a.Hq + h * G + (rr & (G - 1))) * D + lane * EPT, acc);
         }
       }

@@ -199,3 +199,45 @@ def test_scores_below_fp32_weigh_all_keys_alike(amp, gk, dtype):
         _force_runs(be, meta, runs, 6)
         _check(be._forward_prefill(to_dev(q, dtype), None, None, 0, meta), refs, dtype, D, 700)
     assert _device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("gv", [2.0 ** 100, 2.0 ** -100, 2.0 ** 65])
+def test_value_scales_at_the_ends_of_their_range(gv, dtype):
+    """Values of 2,000 * v_scale over many keys: sums of them pass fp32's end, their means do not."""
+    from minisgl_b200 import B200AttnBackend
+
+    Hq, Hkv, D = 4, 2, 128
+    lens, ext = np.array([5000, 60, 1]), np.array([3, 60, 1])
+    big = 2000 * np.sign(np.random.default_rng(0).standard_normal((1, Hkv, D)) + 1.0)
+    p = Pool(lens, Hkv, D, dtype, 16, seed=8, gv=gv, k=1.0, v=big)  # every key weighs 2^7
+    q = rand(p.rng, (int(ext.sum()), Hq, D), dtype)
+    be = B200AttnBackend(HeadConfig(Hq, Hkv, D), p.cache, p.pb.page_table, 16)
+    last = np.cumsum(ext) - 1
+    refs = _refs(p, q[last].astype(np.float64), lens, [1] * 3, be.scale)
+    for nc in (None, 1, 2):
+        out = be.forward_decode(to_dev(q[last], dtype), 0, be.decode_metadata_from_lens(p.pb.rows, p.pb.lens, num_ctas=nc))
+        _check(out, refs, dtype, D, 5000)
+    refs = _refs(p, q.astype(np.float64), lens, ext, be.scale)
+    for runs in (None, 640):
+        meta = be.extend_metadata_from_lens(p.pb.rows, lens, ext)
+        _force_runs(be, meta, runs, 8)
+        _check(be._forward_prefill(to_dev(q, dtype), None, None, 0, meta), refs, dtype, D, 5000)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("gk,gv,amp", [(2.0 ** -10, 64.0, 2.0 ** 10), (4.0, 2.0 ** -20, 1.0)])
+def test_extend_over_scaled_pools(gk, gv, amp, dtype):
+    from minisgl_b200 import B200AttnBackend
+
+    Hq, Hkv, D = 16, 8, 128
+    lens, ext = np.array([700, 90, 200]), np.array([130, 3, 200])
+    p = Pool(lens, Hkv, D, dtype, 16, seed=2, gk=gk, gv=gv)
+    q = rand(p.rng, (int(ext.sum()), Hq, D), dtype) * np.float32(amp)
+    be = B200AttnBackend(HeadConfig(Hq, Hkv, D), p.cache, p.pb.page_table, 16)
+    refs = _refs(p, q.astype(np.float64), lens, ext, be.scale)
+    for runs in (None, 256):
+        meta = be.extend_metadata_from_lens(p.pb.rows, lens, ext)
+        _force_runs(be, meta, runs, 3)
+        _check(be._forward_prefill(to_dev(q, dtype), None, None, 0, meta), refs, dtype, D, 700)
+    assert _device_error() == 0
