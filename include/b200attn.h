@@ -431,9 +431,14 @@ int b2a_fp4_decode(const void* q, const void* pool, int64_t num_slots, const int
  * 128), at most n_split (1 to 64) of them, the last one taking what is left:
  * b2a_fp4_extend_runs (host only) proposes both for items whose last token sees
  * tile_keys[i] keys (host array), n_split 1 when the items fill the GPU anyway.
- * With n_split > 1 the call needs a 256-byte aligned workspace of
- * b2a_fp4_extend_workspace_bytes: merge counters (int32 [n_work * Hkv], zeroed
- * once when it is allocated, zero again after every call), then partial rows.
+ * With n_split > 1 the call needs a 256-byte aligned workspace: merge counters
+ * (int32 [n_work * Hkv], zeroed once when it is allocated, zero again after every
+ * call), then partial rows. b2a_fp4_extend_workspace_bytes has n_split places for
+ * every item, which uneven items leave mostly empty. b2a_fp4_extend_packed_bytes
+ * has n_runs of them: the sum of min(n_split, ceil(keys / run_keys)) over the
+ * items with two runs or more. Any size from the packed size of 2 runs is taken,
+ * with the same results: items that find no place in it are not cut, or into
+ * fewer runs.
  * One workspace serves calls that are ordered on the GPU and have the same
  * n_work and Hkv; it is not shared with b2a_fp4_decode.
  * ------------------------------------------------------------------------ */
@@ -441,6 +446,7 @@ int b2a_fp4_extend_tile_q(int Hq, int Hkv, int D, int dtype, int* tile_q);
 int b2a_fp4_extend_runs(const int32_t* tile_keys, int n_work, int Hq, int Hkv, int D, int dtype, int* run_keys,
                         int* n_split);
 size_t b2a_fp4_extend_workspace_bytes(int n_work, int n_split, int Hkv, int D);
+size_t b2a_fp4_extend_packed_bytes(int n_work, int n_runs, int Hkv, int D, int dtype);
 int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int32_t* qo_indptr,
                    const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* kv_last_page_len, int page_size,
                    const int32_t* work, int n_work, int run_keys, int n_split, int T, int B, int Hq, int Hkv, int D,

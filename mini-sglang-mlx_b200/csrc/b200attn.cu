@@ -1321,6 +1321,12 @@ size_t b2a_fp4_extend_workspace_bytes(int n_work, int n_split, int Hkv, int D) {
   return align256(items * sizeof(int32_t)) + items * n_split * b2a::kF4Rows * (size_t)(D + 2) * sizeof(float);
 }
 
+size_t b2a_fp4_extend_packed_bytes(int n_work, int n_runs, int Hkv, int D, int dtype) {
+  if (n_work <= 0 || n_runs <= 1 || Hkv <= 0 || D <= 0) return 0;
+  return align256((size_t)n_work * Hkv * sizeof(int32_t)) +
+         (size_t)n_runs * Hkv * b2a::extend_fp4_rows(D, dtype == B2A_DTYPE_F32) * (size_t)(D + 2) * sizeof(float);
+}
+
 int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int32_t* qo_indptr,
                    const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* kv_last_page_len, int page_size,
                    const int32_t* work, int n_work, int run_keys, int n_split, int T, int B, int Hq, int Hkv, int D,
@@ -1343,8 +1349,9 @@ int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int
     return fail(B2A_ERR_INVALID, "q/pool/out must be 16-byte aligned");
   if (num_slots <= 0 || num_slots > 0x7fffffffLL) return fail(B2A_ERR_INVALID, "num_slots must be in (0, 2^31)");
   const size_t need = b2a_fp4_extend_workspace_bytes(n_work, n_split, Hkv, D);
-  if (need > 0 && (!workspace || workspace_bytes < need))
-    return fail(B2A_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  const size_t least = n_split > 1 ? b2a_fp4_extend_packed_bytes(n_work, 2, Hkv, D, dtype) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < least))
+    return fail(B2A_ERR_WORKSPACE, "workspace of at least %zu bytes needed, %zu given", least, workspace_bytes);
   if (workspace && !aligned(workspace, 256)) return fail(B2A_ERR_INVALID, "workspace must be 256-byte aligned");
   const int G = Hq / Hkv;
   b2a::F4Args a = {};
@@ -1359,8 +1366,16 @@ int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int
   if (need > 0) {
     const size_t items = (size_t)n_work * Hkv;
     a.tickets = reinterpret_cast<int32_t*>(workspace);
-    a.ws_acc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + align256(items * sizeof(int32_t)));
-    a.ws_ml = a.ws_acc + items * n_split * b2a::kF4Rows * (size_t)D;
+    const size_t counters = align256(items * sizeof(int32_t));
+    a.ws_acc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + counters);
+    const size_t rows = (size_t)b2a::extend_fp4_rows(D, dtype == B2A_DTYPE_F32);
+    size_t runs = items * n_split;  // of all heads
+    if (workspace_bytes < need) {
+      const size_t fit = (workspace_bytes - counters) / (Hkv * rows * (size_t)(D + 2) * sizeof(float));
+      a.ws_runs = (int)std::min<size_t>(fit, 1u << 30);
+      runs = (size_t)a.ws_runs * Hkv;
+    }
+    a.ws_ml = a.ws_acc + runs * rows * (size_t)D;
   }
   a.num_slots = num_slots;
   a.row_bytes = b2a::fp4_row_bytes(Hkv, D);
@@ -1380,7 +1395,7 @@ int b2a_fp4_extend(const void* q, const void* pool, int64_t num_slots, const int
     constexpr bool F32 = std::is_same<decltype(tag), float>::value;
     return with_d(D, [&](auto dc) -> int {
       constexpr int Dc = decltype(dc)::value;
-      auto kern = b2a::extend_fp4_tc_kernel<Dc, F32>;
+      auto kern = a.ws_runs > 0 ? b2a::extend_fp4_tc_kernel<Dc, F32, true> : b2a::extend_fp4_tc_kernel<Dc, F32, false>;
       constexpr size_t smem = b2a::F4Cfg<Dc, F32>::ALLOC;
       if (int rc = ensure_smem((const void*)kern, smem, "fp4_extend")) return rc;
       // grid order as extend_tc.cuh: heads innermost, cost-sorted items behind them, runs outermost

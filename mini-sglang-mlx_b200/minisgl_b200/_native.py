@@ -119,6 +119,7 @@ SIGNATURES = {
     "b2a_fp4_extend_runs": (
         c_int, [_P, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_int), ctypes.POINTER(c_int)]),
     "b2a_fp4_extend_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "b2a_fp4_extend_packed_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "b2a_extend_metadata": (
         c_int,
         [_P, c_int64, c_int64, _P, _P, _P, c_int, c_int, c_int, _P, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P,
@@ -216,6 +217,25 @@ def fp4_extend_runs(tile_keys: np.ndarray, Hq: int, Hkv: int, D: int, dtype_code
     run, n = c_int(0), c_int(1)
     call("b2a_fp4_extend_runs", np_ptr(keys), keys.size, Hq, Hkv, D, dtype_code, ctypes.byref(run), ctypes.byref(n))
     return run.value, n.value
+
+
+FP4_WHOLE_WORKSPACE = 64 << 20
+
+
+def fp4_extend_workspace(tile_keys: np.ndarray, n_work: int, run_keys: int, n_split: int, Hkv: int, D: int,
+                         dtype_code: int) -> int:
+    """Workspace bytes of an extend over the 4-bit pool whose work items see ``tile_keys`` keys.
+
+    Places for every item's n_split runs while they take 64 MB at most, else the batch's own
+    runs, packed (b2a_fp4_extend_packed_bytes; 2 us a call): one long request among many short
+    ones has many more places than runs (83 requests of 300 keys and one of 32,768 on one kv head:
+    716 MB of places for 8.5 MB of runs).
+    """
+    whole = int(LIB.b2a_fp4_extend_workspace_bytes(n_work, n_split, Hkv, D))
+    if whole <= FP4_WHOLE_WORKSPACE:
+        return whole
+    runs = np.minimum(-(-np.asarray(tile_keys, dtype=np.int64) // run_keys), n_split)
+    return min(whole, int(LIB.b2a_fp4_extend_packed_bytes(n_work, max(2, int(runs[runs > 1].sum())), Hkv, D, dtype_code)))
 
 
 def extend_plan(qo_indptr: np.ndarray, kv_indptr: np.ndarray, kv_last_page_len: np.ndarray | None,

@@ -306,7 +306,8 @@ class B200AttnBackend(BaseAttnBackend):
         """Cut the keys of few work items into runs (4-bit pool), with a workspace of the batch's own."""
         with self._here():
             meta.run_keys, meta.n_split = nat.fp4_extend_runs(tile_keys, self.Hq, self.Hkv, self.D, self.dtype_code)
-            nbytes = int(nat.LIB.b2a_fp4_extend_workspace_bytes(meta.n_work, meta.n_split, self.Hkv, self.D))
+            nbytes = nat.fp4_extend_workspace(tile_keys, meta.n_work, meta.run_keys, meta.n_split, self.Hkv, self.D,
+                                              self.dtype_code)
             if nbytes:
                 meta.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
                 meta.workspace[: 4 * meta.n_work * self.Hkv].zero_()  # the merge counters at its start

@@ -241,3 +241,74 @@ def test_extend_over_scaled_pools(gk, gv, amp, dtype):
         _force_runs(be, meta, runs, 3)
         _check(be._forward_prefill(to_dev(q, dtype), None, None, 0, meta), refs, dtype, D, 700)
     assert _device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,D", [("bfloat16", 128), ("float32", 128), ("bfloat16", 256), ("float32", 64)])
+def test_extend_in_a_packed_workspace(dtype, D):
+    """Workspaces of any size between two runs and all of them: items are cut as far as it goes, the
+    rows agree with float64, a second call on the same workspace repeats them, and nothing is written behind it."""
+    import torch
+
+    from minisgl_b200 import B200AttnBackend
+    from minisgl_b200 import _native as nat
+
+    Hq, Hkv = 4, 2
+    lens = np.array([40, 700, 33, 1100, 300, 64, 513])
+    ext = np.array([40, 5, 1, 200, 2, 64, 90])
+    p = Pool(lens, Hkv, D, dtype, 16, seed=9)
+    q = rand(p.rng, (int(ext.sum()), Hq, D), dtype)
+    qd = to_dev(q, dtype)
+    be = B200AttnBackend(HeadConfig(Hq, Hkv, D), p.cache, p.pb.page_table, 16)
+    refs = _refs(p, q.astype(np.float64), lens, ext, be.scale)
+    meta = be.extend_metadata_from_lens(p.pb.rows, lens, ext)
+    w = meta.work.cpu().numpy()
+    keys = (lens - ext)[w[:, 0]] + w[:, 1] + w[:, 2]
+    meta.run_keys, meta.n_split = 128, 9
+    runs = np.minimum(-(-keys // 128), 9)
+    total = int(runs[runs > 1].sum())
+    code = be.dtype_code
+    n_all = int(nat.LIB.b2a_fp4_extend_workspace_bytes(meta.n_work, 9, Hkv, D))
+    sizes = [int(nat.LIB.b2a_fp4_extend_packed_bytes(meta.n_work, r, Hkv, D, code)) for r in (2, 3, 7, total - 1, total)]
+    outs = []
+    for n in [*sizes, sizes[-1] + 64, n_all - 4, n_all]:
+        buf = torch.zeros(n + 4096, dtype=torch.uint8, device="cuda")
+        buf[n:] = 0x5A
+        meta.workspace = buf[:n]
+        first = be._forward_prefill(qd, None, None, 0, meta)
+        assert bool((be._forward_prefill(qd, None, None, 0, meta) == first).all()), "extend is not repeatable"
+        _check(first, refs, dtype, D, int(lens.max()))
+        assert (buf[n:] == 0x5A).all(), "written behind the workspace"
+        assert (buf[: 4 * meta.n_work * Hkv] == 0).all(), "merge counters are not re-armed"
+        outs.append(first)
+    assert all(bool((o == outs[-1]).all()) for o in outs[4:])  # the same runs, wherever their rows lie
+    meta.workspace = torch.zeros(sizes[0] - 4, dtype=torch.uint8, device="cuda")
+    with pytest.raises(nat.B200AttnError):
+        be._forward_prefill(qd, None, None, 0, meta)
+    assert _device_error() == 0
+
+
+def test_one_long_request_among_short_ones_through_the_backend():
+    """Tables of both builders ask for the batch's own runs only, and attend alike."""
+    import torch
+
+    from minisgl_b200 import B200AttnBackend
+
+    Hq, Hkv, D, P = 2, 1, 128, 16
+    lens = np.array([300] * 40 + [20000] + [300] * 43)
+    ext = np.where(lens > 300, 3, 128)
+    p = Pool(lens, Hkv, D, "bfloat16", P, seed=1)
+    be = B200AttnBackend(HeadConfig(Hq, Hkv, D), p.cache, p.pb.page_table, P)
+    q = to_dev(rand(p.rng, (int(ext.sum()), Hq, D), "bfloat16"), "bfloat16")
+    host = be.extend_metadata_from_lens(p.pb.rows, lens, ext)
+    assert host.n_split > 8 and host.workspace.numel() <= 64 << 20
+    want = be._forward_prefill(q, None, None, 0, host)
+    o = int(ext[:40].sum())
+    ref = F.attend(q[o:o + 3].double().cpu().numpy(), *p.of(40), be.scale, 20000 - 3)
+    _check(want[o:o + 3], [ref], "bfloat16", D, 20000)
+    meta = be.alloc_extend_metadata(84, int(ext.sum()), int(((lens + P - 1) // P).sum()), cached=lens - ext, lens=lens)
+    assert meta.workspace.numel() <= 64 << 20
+    be.build_extend_metadata_device(meta, _i32(p.pb.page_table), _i32(p.pb.rows), _i32(lens - ext), _i32(lens))
+    for _ in range(2):
+        assert bool((be._forward_prefill(q, None, None, 0, meta) == want).all())
+    assert _device_error() == 0
+    torch.cuda.empty_cache()
