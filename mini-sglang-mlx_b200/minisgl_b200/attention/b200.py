@@ -114,6 +114,10 @@ class B200AttnBackend(BaseAttnBackend):
         self._stage: tuple | None = None  # packed K/V staging pools for small-page prefill
         self._tiles: dict = {}  # page size -> query tokens of an extend tile
         self.fp4 = isinstance(kv_cache, FP4KVCache)  # the pool holds 4-bit rows (kvcache/fp4.py)
+        if self.fp4 and (kv_cache.num_kv_heads, kv_cache.head_dim) != (self.Hkv, self.D):
+            # a row's length follows from them: another shape's rows would be read past the pool's end
+            raise ValueError(f"the 4-bit pool holds {kv_cache.num_kv_heads} kv heads of {kv_cache.head_dim} features, "
+                             f"the model has {self.Hkv} of {self.D}")
         n = nat.ctypes.c_int(0)
         with torch.cuda.device(self.device):
             nat.call("b2a_fp4_decode_num_ctas" if self.fp4 else "b2a_decode_num_ctas", self.Hq, self.Hkv, self.D, self.dtype_code, nat.ctypes.byref(n))

@@ -312,3 +312,14 @@ def test_one_long_request_among_short_ones_through_the_backend():
         assert bool((be._forward_prefill(q, None, None, 0, meta) == want).all())
     assert _device_error() == 0
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("Hkv,D", [(4, 128), (8, 64), (16, 128), (8, 256)])
+def test_a_pool_of_another_shape_is_refused(Hkv, D):
+    import torch
+
+    from minisgl_b200 import B200AttnBackend, FP4KVCache
+
+    cache = FP4KVCache(1, 64, Hkv, D, torch.bfloat16, "cuda")
+    with pytest.raises(ValueError, match="kv heads"):
+        B200AttnBackend(HeadConfig(16, 8, 128), cache, np.zeros((1, 64), np.int32), 16)
