@@ -111,6 +111,7 @@ class B200AttnBackend(BaseAttnBackend):
         self._page_size = page_size
         self._stager = PinnedStager()
         self._workspace = torch.empty(0, dtype=torch.uint8, device=self.device)
+        self._retired: list = []  # workspaces that larger ones replaced: each at most half of the next
         self._stage: tuple | None = None  # packed K/V staging pools for small-page prefill
         self._tiles: dict = {}  # page size -> query tokens of an extend tile
         self.fp4 = isinstance(kv_cache, FP4KVCache)  # the pool holds 4-bit rows (kvcache/fp4.py)
@@ -147,6 +148,8 @@ class B200AttnBackend(BaseAttnBackend):
         # zero-filled once: the merge counters at its start must be zero before the
         # first decode call, and every call leaves them at zero again
         if self._workspace.numel() < nbytes:
+            if self._workspace.numel():
+                self._retired.append(self._workspace)  # a captured graph may still write to it
             self._workspace = torch.zeros(max(nbytes, 2 * self._workspace.numel()), dtype=torch.uint8,
                                           device=self.device)
         return self._workspace

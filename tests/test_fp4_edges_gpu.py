@@ -323,3 +323,29 @@ def test_a_pool_of_another_shape_is_refused(Hkv, D):
     cache = FP4KVCache(1, 64, Hkv, D, torch.bfloat16, "cuda")
     with pytest.raises(ValueError, match="kv heads"):
         B200AttnBackend(HeadConfig(16, 8, 128), cache, np.zeros((1, 64), np.int32), 16)
+
+
+def test_a_captured_decode_keeps_its_workspace():
+    """A decode captured with host-built metadata goes on after a larger batch has replaced the workspace."""
+    import weakref
+
+    import torch
+
+    from minisgl_b200 import B200AttnBackend
+
+    lens = [900, 70]
+    p = Pool(lens, 8, 128, "bfloat16", 16, seed=4)
+    be = B200AttnBackend(HeadConfig(16, 8, 128), p.cache, p.pb.page_table, 16)
+    q = to_dev(rand(p.rng, (2, 16, 128), "bfloat16"), "bfloat16")
+    meta = be.decode_metadata_from_lens(p.pb.rows, p.pb.lens, num_ctas=8)
+    want = be.forward_decode(q, 0, meta)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = be.forward_decode(q, 0, meta)
+    used = weakref.ref(be._workspace)
+    big = be.decode_metadata_from_lens(p.pb.rows, p.pb.lens, num_ctas=31)
+    be.forward_decode(q, 0, big)
+    assert be._workspace is not used() and used() is not None, "the captured workspace was given back"
+    g.replay()
+    torch.cuda.synchronize()
+    assert bool((out == want).all())
