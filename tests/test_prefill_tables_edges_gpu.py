@@ -249,3 +249,69 @@ def test_work_lists_of_known_batches_are_exact(pool):
     for bad in (-1, T + 5):
         with pytest.raises(ValueError, match="tiles"):
             be.alloc_extend_metadata(4, T, NP, n_work=bad)
+
+
+@pytest.mark.parametrize("short", ["tokens", "pages", "tiles", "nothing"])
+def test_nothing_is_written_past_a_buffer(short):
+    """Buffers that lie between guard words, at and one below the size the batch needs."""
+    import torch
+
+    lens, cached = np.array([300, 90, 17, 4000]), np.array([0, 80, 16, 3990])
+    be, pb, _ = _backend(lens)
+    T, NP = int((lens - cached).sum()), int(((lens + P - 1) // P).sum())
+    tiles = be.extend_tiles(cached, lens)
+    n = dict(positions=T - (short == "tokens"), out_loc=T - (short == "tokens"), kv_indices=NP - (short == "pages"),
+             work=4 * (tiles - (short == "tiles")), qo_indptr=5, kv_indptr=5, last_indices=4, kv_last_page_len=4, counts=2)
+    meta = be.alloc_extend_metadata(4, T, NP, n_work=tiles)
+    bufs = {}
+    for name, size in n.items():
+        b = torch.full((64 + size + 64,), 0x5A5A, dtype=torch.int32, device="cuda")  # 256 bytes of guard: work stays aligned
+        bufs[name] = b
+        t = b[64: 64 + size]
+        setattr(meta, name, t.view(-1, 4) if name == "work" else t)
+    meta.n_work = n["work"] // 4
+    be.build_extend_metadata_device(meta, _i32(pb.page_table), _i32(pb.rows), _i32(cached), _i32(lens))
+    assert _device_error() == (0 if short == "nothing" else 34)
+    for name, b in bufs.items():
+        assert (b[:64] == 0x5A5A).all() and (b[64 + n[name]:] == 0x5A5A).all(), name
+    if short == "nothing":
+        host = be.extend_metadata_from_lens(pb.rows, lens, lens - cached)
+        for name in ("qo_indptr", "kv_indptr", "kv_indices", "kv_last_page_len", "work", "last_indices"):
+            assert bool((getattr(meta, name) == getattr(host, name)).all()), name
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("lengths", ["known", "unknown"])
+def test_long_prefixes_in_runs_behind_device_tables(lengths, dtype):
+    """Keys cut into runs from host copies of the lengths or from a guess of equal ones, with empty tiles
+    in the list: the float64 attention, again on a second call, and after other lengths used the buffers."""
+    import torch
+
+    from oracle import fp4 as F
+
+    lens, cached = np.array([6000, 3100]), np.array([5990, 3099])
+    be, pb, rng = _backend(lens, "fp4", dtype)
+    cache = be.kv_cache
+    k, v = (rand(rng, (pb.num_slots, HKV, D), dtype) for _ in range(2))
+    cache.store_kv(to_dev(k, dtype), to_dev(v, dtype), _i32(np.arange(pb.num_slots)), 0)
+    kr, vr = F.roundtrip(k), F.roundtrip(v)
+    T, NP = 40, int(((lens + P - 1) // P).sum())
+    kw = dict(cached=cached, lens=lens) if lengths == "known" else {}
+    meta = be.alloc_extend_metadata(2, T, NP, **kw)
+    assert meta.n_split > 1
+    table, rows = _i32(pb.page_table), _i32(pb.rows)
+    q = rand(rng, (T, HQ, D), dtype)
+    for c2, n2 in ((cached, lens), (np.array([4980, 100]), np.array([5000, 120])), (cached, lens)):
+        be.build_extend_metadata_device(meta, table, rows, _i32(c2), _i32(n2))
+        out = be._forward_prefill(to_dev(q, dtype), None, None, 0, meta)
+        again = be._forward_prefill(to_dev(q, dtype), None, None, 0, meta)
+        o = 0
+        for b in range(2):
+            m = int(n2[b] - c2[b])
+            s = pb.page_table[b, : int(n2[b])]
+            ref, A, X, S = F.attend(q[o:o + m].astype(np.float64), kr[s], vr[s], be.scale, int(c2[b]))
+            got = out[o:o + m].double().cpu().numpy()
+            assert (np.abs(got - ref) <= F.tolerance(ref, A, X, S, dtype, D, int(n2[b]))).all()
+            o += m
+        assert bool((out[:o] == again[:o]).all()), "extend is not repeatable"
+    assert _device_error() == 0
