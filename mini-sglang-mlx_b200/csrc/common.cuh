@@ -14,7 +14,6 @@ namespace b2a {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr float kNaN = __builtin_nanf("");
 
 // Watchdog word: a bounded wait that gives up writes a nonzero code here and
 // the kernel unwinds. Read (and cleared) by b2a_device_error().
@@ -31,10 +30,6 @@ enum WatchdogCode : int {
   kWdMetaOverflow = 34,  // device metadata: a row, length or entry outside its buffer: skipped
   kWdBadPlan = 35,       // decode plan: a request id or partial slot outside its bounds: segment skipped
 };
-
-// A pool slot of -1: this row has none (padding of a captured step), the stores skip it. Any
-// other slot outside the pool is an error (kWdBadSlot).
-constexpr int kNoSlot = -1;
 
 __device__ __forceinline__ void watchdog_set(int code) { atomicCAS(&g_watchdog, 0, code); }
 

@@ -98,6 +98,8 @@ __device__ __forceinline__ void fp4_row_factor(float amax, float& f, float& inv)
   inv = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
 }
 
+constexpr float kNaN = __builtin_nanf("");
+
 // Whether a row's weights are lost, for the weight sum of a row that has seen a key (NaN: shown already).
 __device__ __forceinline__ bool fp4_row_lost(float sum) { return sum < 1.f; }
 

@@ -26,6 +26,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "slot.cuh"
 
 namespace b2a {
 

@@ -28,6 +28,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "slot.cuh"
 
 namespace b2a {
 

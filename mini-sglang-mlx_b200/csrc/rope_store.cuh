@@ -18,6 +18,7 @@
 // written back before the rotation reads it.
 #pragma once
 #include "common.cuh"
+#include "slot.cuh"
 
 namespace b2a {
 
