@@ -100,7 +100,8 @@ __device__ __forceinline__ void fp4_row_factor(float amax, float& f, float& inv)
 
 constexpr float kNaN = __builtin_nanf("");
 
-// Whether a row's weights are lost, for the weight sum of a row that has seen a key (NaN: shown already).
+// Whether a row's weights are lost, for the weight sum of a row that has seen a key: 2^7 less what
+// rounding takes from scores the softmax can tell apart (NaN: shown already).
 __device__ __forceinline__ bool fp4_row_lost(float sum) { return sum < 1.f; }
 
 // Softmax scale of a head row's raw scores, kept above zero: at the smallest normal float every score

@@ -25,7 +25,7 @@
 // of 64 keys so that both parts of P find room beside S.
 //
 // Few rows on long prefixes leave most SMs idle, so the keys of an item can be cut into runs of
-// run_blocks blocks (grid z). Each run writes its unnormalised rows and (m, l) to a workspace;
+// run_keys keys (grid z). Each run writes its unnormalised rows and (m, l) to a workspace;
 // the CTA that takes the item's last ticket joins them, in run order. Nothing waits for another
 // CTA. The rows of run z of an item lie at place z of the item's n_split, or, in a smaller
 // workspace (PACKED), behind the runs of the items before it: every warp of a split item counts
@@ -36,7 +36,7 @@
 // clocks, 2,650 of them without the softmax, 3,900 without the expansion; the MMAs alone are
 // 2,048. The softmax chain of a tile is the longer pole, as in extend_tc.cuh, and every CTA adds
 // about 14,000 clocks of set-up, Q conversion and epilogue. 32 requests of 64 to 512 new tokens
-// on prefixes up to 4,608 run in 256 us (645 TFLOP/s of visible work). A narrow block takes about
+// on prefixes up to 4,608 run in 259 us (637 TFLOP/s of visible work). A narrow block takes about
 // 2,800 clocks, 2,500 of the expanding warps' and the issuers' waits in turn: 8 requests of 1 to
 // 16 new tokens on 6,000 to 16,000 cached ones run in 100 us.
 //

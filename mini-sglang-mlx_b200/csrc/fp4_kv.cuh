@@ -120,8 +120,8 @@ __device__ __forceinline__ void fp4_read16(const T* p, bool vec, float (&x)[16])
 // contiguous over a token's heads. HBM bounds both kernels at large n: a thread takes kFp4Unroll
 // blocks kFp4Threads apart, so that many independent slot -> row reads are in flight, and one
 // 64-bit division per thread finds the first token. Store and load of 16,391 fp32 tokens of
-// 8 x 128 take 71 us (a block and a division per thread: 77), the load of 120,001 bf16 ones
-// 126 us, 5.0 TB/s (149).
+// 8 x 128 take 71.5 us (a block and a division per thread: 77), the load of 120,001 bf16 ones
+// 127 us, 5.0 TB/s (149).
 constexpr int kFp4Threads = 256;
 constexpr int kFp4Unroll = 4;
 

@@ -341,10 +341,14 @@ class B200AttnBackend(BaseAttnBackend):
 
         ``total_q`` new tokens and ``total_pages`` pages in all: what the batch needs, or the
         capacity of a batch whose lengths are known on the device only (a captured step). A batch
-        that needs less leaves the tails of ``positions`` and ``kv_indices`` as they were, -1 (no slot:
-        ``store_kv`` skips the row) in the tail of ``out_loc``, and empty tiles at the end of ``work``. ``tile_q`` defaults to the tile of this
-        backend's extend kernel; tables of a larger one serve other consumers, ``forward`` refuses them. Host copies of ``cached`` and ``lens``, where the caller has
-        them, let a 4-bit pool cut long requests' keys into runs as evenly as
+        that needs less leaves the tails of ``positions`` and ``kv_indices`` as they were, -1 (no
+        slot: ``store_kv`` skips the row) in the tail of ``out_loc``, and empty tiles at the end of
+        ``work``; ``forward`` leaves the output rows behind its last token unwritten. The metadata
+        serves one stream at a time.
+
+        ``tile_q`` defaults to the tile of this backend's extend kernel; tables of a larger one serve
+        other consumers, ``forward`` refuses them. Host copies of ``cached`` and ``lens``, where the
+        caller has them, let a 4-bit pool cut long requests' keys into runs as evenly as
         ``extend_metadata_from_lens`` does; without them it assumes requests of equal length.
         ``n_work`` is the number of tiles where the caller knows it (``extend_tiles``); the default is
         the most that ``total_q`` tokens of ``batch_size`` requests can take.

@@ -63,7 +63,7 @@ class EngineConfig:
     # norms, residual adds and SwiGLU fused in (False: cuBLAS + separate kernels throughout)
     fused_proj: bool = True
     # "auto": the KV pool holds `dtype`; "fp4": 4-bit rows (FP4KVCache), 3.5 times the tokens in
-    # the bytes of a bf16 pool
+    # the bytes of a bf16 pool (its scales at 1: blocks of keys or values below 0.006 are stored as 0)
     kv_cache_dtype: str = "auto"
     seed: int = 42
 
